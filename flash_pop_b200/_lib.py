@@ -41,6 +41,7 @@ NVCC_FLAGS = [
 FPB_BF16, FPB_F32 = 0, 1
 STATIC_SCRATCH_BYTES = 16 << 20      # FPB_STATIC_SCRATCH_BYTES of the header
 PATH_NONE, PATH_SIMT, PATH_TCGEN05 = 0, 1, 2
+QK_NORM_SLABS = 592                  # FPB_QK_NORM_SLABS of the header
 FLAG_FORCE_SIMT, FLAG_SKIP_DQ, FLAG_SKIP_DKDV, FLAG_STATE_F32 = 1, 2, 4, 8
 
 
@@ -194,6 +195,20 @@ _SIGNATURES = {
     "fpb_gate_residual_bwd": [ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
                               ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
                               ctypes.c_void_p],
+    "fpb_qk_norm_rotary_fwd": [ctypes.c_int32] * 6 + [ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+                               _SEQ_P, _SEQ_P, _SEQ_P, _SEQ_P, ctypes.c_void_p],
+    "fpb_qk_norm_rotary_bwd": [ctypes.c_int32] * 6 + [ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+                               _SEQ_P, _SEQ_P, _SEQ_P, _SEQ_P, _SEQ_P, _SEQ_P, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                               ctypes.c_void_p],
+    "fpb_dropout": [ctypes.c_int64, ctypes.c_int32, ctypes.c_double] + [ctypes.c_void_p] * 5,
+    "fpb_embedding_fwd": [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+                          ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p],
+    "fpb_embedding_bwd": [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64, ctypes.c_float,
+                          ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p],
+    "fpb_token_scores_fwd": [ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64] +
+                            [ctypes.c_void_p] * 7,
+    "fpb_token_scores_bwd": [ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64] +
+                            [ctypes.c_void_p] * 8 + [ctypes.c_int64, ctypes.c_void_p],
     "fpb_device_status": [ctypes.c_void_p, ctypes.POINTER(ctypes.c_int32)],
 }
 # hooks of the diagnostics build only
@@ -215,7 +230,7 @@ _DIAG_SIGNATURES = {
 def exported_symbols() -> list[str]:
     """Every entry point include/flash_pop_b200.h declares."""
     return list(_SIGNATURES) + ["fpb_strerror", "fpb_version", "fpb_last_path", "fpb_last_cuda_error",
-                                "fpb_launch_count", "fpb_workspace_bytes", "fpb_decoder_token_workspace"]
+                                "fpb_launch_count", "fpb_workspace_bytes", "fpb_decoder_token_workspace", "fpb_embedding_workspace"]
 
 
 def _load(path: str) -> ctypes.CDLL:
@@ -238,6 +253,8 @@ def _load(path: str) -> ctypes.CDLL:
     handle.fpb_workspace_bytes.restype = ctypes.c_int64
     handle.fpb_decoder_token_workspace.argtypes = [ctypes.POINTER(_TokenDims)]
     handle.fpb_decoder_token_workspace.restype = ctypes.c_int64
+    handle.fpb_embedding_workspace.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32]
+    handle.fpb_embedding_workspace.restype = ctypes.c_int64
     return handle
 
 

@@ -706,6 +706,154 @@ int fpb_cross_entropy_bwd(int64_t rows, int32_t V, int32_t dtype, const void* lo
   return finish_launches(1, -1);
 }
 
+namespace {
+int check_qk_norm(int32_t B, int32_t T, int32_t Hq, int32_t Hk, int32_t d, int32_t dtype, const float* w_q, const float* w_k,
+                  const float* phasors, int64_t phasor_stride_b) {
+  if (B < 0 || T < 0 || Hq < 0 || Hk < 0 || d <= 0 || d % 8 || d > 256) return FPB_ERR_BAD_SHAPE;
+  if (!dtype_ok(dtype)) return FPB_ERR_BAD_DTYPE;
+  if ((uintptr_t)w_q % 16 || (uintptr_t)w_k % 16 || (uintptr_t)phasors % 16 || phasor_stride_b % 2 || phasor_stride_b < 0) return FPB_ERR_BAD_STRIDE;
+  return FPB_OK;
+}
+}  // namespace
+
+int fpb_qk_norm_rotary_fwd(int32_t B, int32_t T, int32_t Hq, int32_t Hk, int32_t d, int32_t dtype, float eps, const float* w_q,
+                           const float* w_k, const float* phasors, int64_t phasor_stride_b, const fpb_seq* q, const fpb_seq* k,
+                           const fpb_seq* q_out, const fpb_seq* k_out, fpb_stream_t stream) {
+  FPB_TRY(check_qk_norm(B, T, Hq, Hk, d, dtype, w_q, w_k, phasors, phasor_stride_b));
+  FPB_TRY(check_plain_seq(q, dtype, B, T, Hq, d, 16)); FPB_TRY(check_plain_seq(k, dtype, B, T, Hk, d, 16));
+  FPB_TRY(check_plain_seq(q_out, dtype, B, T, Hq, d, 16)); FPB_TRY(check_plain_seq(k_out, dtype, B, T, Hk, d, 16));
+  FPB_TRY(check_device());
+  if ((int64_t)B * T == 0 || (int64_t)Hq + Hk == 0) return FPB_OK;
+  const SeqView x[2] = {view(q), view(k)}, out[2] = {view(q_out), view(k_out)};
+  const float* w[2] = {w_q, w_k};
+  float* none[2] = {nullptr, nullptr};
+  const int r = launch_qk_norm(dtype, false, B, T, Hq, Hk, d, eps, w, phasors, phasor_stride_b, x, nullptr, out, none, nullptr, (cudaStream_t)stream);
+  const int f = finish_launches(1, -1);
+  return r != FPB_OK ? r : f;
+}
+
+int fpb_qk_norm_rotary_bwd(int32_t B, int32_t T, int32_t Hq, int32_t Hk, int32_t d, int32_t dtype, float eps, const float* w_q,
+                           const float* w_k, const float* phasors, int64_t phasor_stride_b, const fpb_seq* q, const fpb_seq* k,
+                           const fpb_seq* d_yq, const fpb_seq* d_yk, const fpb_seq* d_q, const fpb_seq* d_k, float* d_w_q, float* d_w_k,
+                           void* scratch, fpb_stream_t stream) {
+  FPB_TRY(check_qk_norm(B, T, Hq, Hk, d, dtype, w_q, w_k, phasors, phasor_stride_b));
+  FPB_TRY(check_plain_seq(q, dtype, B, T, Hq, d, 16)); FPB_TRY(check_plain_seq(k, dtype, B, T, Hk, d, 16));
+  FPB_TRY(check_plain_seq(d_yq, dtype, B, T, Hq, d, 16)); FPB_TRY(check_plain_seq(d_yk, dtype, B, T, Hk, d, 16));
+  FPB_TRY(check_plain_seq(d_q, dtype, B, T, Hq, d, 16)); FPB_TRY(check_plain_seq(d_k, dtype, B, T, Hk, d, 16));
+  if (!scratch) return FPB_ERR_NULL_POINTER;
+  if ((uintptr_t)scratch % 16) return FPB_ERR_BAD_WORKSPACE;
+  FPB_TRY(check_device());
+  if ((int64_t)B * T == 0 || (int64_t)Hq + Hk == 0) {            // sums over no rows
+    if ((d_w_q && cudaMemsetAsync(d_w_q, 0, sizeof(float) * d, (cudaStream_t)stream) != cudaSuccess) ||
+        (d_w_k && cudaMemsetAsync(d_w_k, 0, sizeof(float) * d, (cudaStream_t)stream) != cudaSuccess))
+      return finish_launches(0, -1);
+    return FPB_OK;
+  }
+  const SeqView x[2] = {view(q), view(k)}, dy[2] = {view(d_yq), view(d_yk)}, out[2] = {view(d_q), view(d_k)};
+  const float* w[2] = {w_q, w_k};
+  float* dw[2] = {d_w_q, d_w_k};
+  const int r = launch_qk_norm(dtype, true, B, T, Hq, Hk, d, eps, w, phasors, phasor_stride_b, x, dy, out, dw, (float*)scratch, (cudaStream_t)stream);
+  const int f = finish_launches(d_w_q || d_w_k ? 2 : 1, -1);
+  return r != FPB_OK ? r : f;
+}
+
+int fpb_dropout(int64_t n, int32_t dtype, double p, const int64_t* seed, const void* x, const void* residual, void* y, fpb_stream_t stream) {
+  if (n < 0 || !(p >= 0.0 && p <= 1.0)) return FPB_ERR_BAD_SHAPE;
+  if (n >= (1ll << 40)) return FPB_ERR_TOO_LARGE;
+  if (!dtype_ok(dtype)) return FPB_ERR_BAD_DTYPE;
+  if (n > 0 && (!seed || !x || !y)) return FPB_ERR_NULL_POINTER;
+  const int size = dtype == FPB_F32 ? 4 : 2;
+  if ((uintptr_t)seed % 8 || (uintptr_t)x % size || (uintptr_t)residual % size || (uintptr_t)y % size) return FPB_ERR_BAD_STRIDE;
+  FPB_TRY(check_device());
+  if (n == 0) return FPB_OK;
+  const int r = launch_dropout(dtype, n, p, seed, x, residual, y, (cudaStream_t)stream);
+  const int f = finish_launches(1, -1);
+  return r != FPB_OK ? r : f;
+}
+
+namespace {
+int check_embedding(int64_t N, int64_t V, int32_t D, int32_t dtype, const int64_t* tokens) {
+  if (N < 0 || V <= 0 || D <= 0) return FPB_ERR_BAD_SHAPE;
+  if (N >= (1ll << 31) || V >= (1ll << 31)) return FPB_ERR_TOO_LARGE;
+  if (!dtype_ok(dtype)) return FPB_ERR_BAD_DTYPE;
+  if (N > 0 && !tokens) return FPB_ERR_NULL_POINTER;
+  return (uintptr_t)tokens % 8 ? FPB_ERR_BAD_STRIDE : FPB_OK;
+}
+}  // namespace
+
+int fpb_embedding_fwd(int64_t N, int64_t V, int32_t D, int32_t dtype, const int64_t* tokens, const void* weight, int64_t w_stride,
+                      float scale, void* y, fpb_stream_t stream) {
+  FPB_TRY(check_embedding(N, V, D, dtype, tokens));
+  if (N > 0 && (!weight || !y)) return FPB_ERR_NULL_POINTER;
+  const int size = dtype == FPB_F32 ? 4 : 2;
+  if ((V > 1 && w_stride < D) || (uintptr_t)weight % size || (uintptr_t)y % size) return FPB_ERR_BAD_STRIDE;
+  FPB_TRY(check_device());
+  if (N == 0) return FPB_OK;
+  const int r = launch_embedding(dtype, N, V, D, tokens, weight, w_stride, scale, y, (cudaStream_t)stream);
+  const int f = finish_launches(1, -1);
+  return r != FPB_OK ? r : f;
+}
+
+int64_t fpb_embedding_workspace(int64_t N, int64_t V, int32_t D) { return embedding_workspace(N, V, D); }
+
+int fpb_embedding_bwd(int64_t N, int64_t V, int32_t D, int32_t dtype, const int64_t* tokens, int64_t padding, float scale, const void* d_y,
+                      int64_t dy_stride, void* d_weight, void* workspace, int64_t workspace_bytes, fpb_stream_t stream) {
+  FPB_TRY(check_embedding(N, V, D, dtype, tokens));
+  if (!d_weight || (N > 0 && !d_y)) return FPB_ERR_NULL_POINTER;
+  const int size = dtype == FPB_F32 ? 4 : 2;
+  if ((N > 1 && dy_stride < D) || (uintptr_t)d_y % size || (uintptr_t)d_weight % size) return FPB_ERR_BAD_STRIDE;
+  if (N > 0 && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < embedding_workspace(N, V, D))) return FPB_ERR_BAD_WORKSPACE;
+  FPB_TRY(check_device());
+  if (N == 0) {
+    if (cudaMemsetAsync(d_weight, 0, (size_t)V * D * size, (cudaStream_t)stream) != cudaSuccess) return finish_launches(0, -1);
+    return FPB_OK;
+  }
+  int n_launched = 0;
+  const int r = launch_embedding_grad(dtype, N, V, D, tokens, padding, scale, d_y, dy_stride, d_weight, workspace, (cudaStream_t)stream, &n_launched);
+  const int f = finish_launches(n_launched, -1);
+  return r != FPB_OK ? r : f;
+}
+
+namespace {
+int check_scores(int64_t rows, int32_t V, int32_t dtype, int32_t top, const void* logits, int64_t row_stride, const int64_t* tokens) {
+  if (rows < 0 || V <= 0 || top < 0 || top > FPB_MAX_TOP || top > V) return FPB_ERR_BAD_SHAPE;
+  if (rows >= (1ll << 31) || V > (1 << 30)) return FPB_ERR_TOO_LARGE;
+  if (!dtype_ok(dtype)) return FPB_ERR_BAD_DTYPE;
+  if (rows == 0) return FPB_OK;
+  if (!logits || !tokens) return FPB_ERR_NULL_POINTER;
+  if ((rows > 1 && row_stride < V) || (uintptr_t)logits % (dtype == FPB_F32 ? 4 : 2) || (uintptr_t)tokens % 8) return FPB_ERR_BAD_STRIDE;
+  return FPB_OK;
+}
+}  // namespace
+
+int fpb_token_scores_fwd(int64_t rows, int32_t V, int32_t dtype, int32_t top, const void* logits, int64_t row_stride, const int64_t* tokens,
+                         float* logprob, float* entropy, float* stats, float* top_logprob, int64_t* top_tokens, fpb_stream_t stream) {
+  FPB_TRY(check_scores(rows, V, dtype, top, logits, row_stride, tokens));
+  if (rows > 0 && (!logprob || !entropy || !stats || (top > 0 && (!top_logprob || !top_tokens)))) return FPB_ERR_NULL_POINTER;
+  if ((uintptr_t)stats % 8) return FPB_ERR_BAD_STRIDE;
+  FPB_TRY(check_device());
+  if (rows == 0) return FPB_OK;
+  const int r = launch_token_scores(dtype, rows, V, top, logits, row_stride, tokens, logprob, entropy, stats, top_logprob, top_tokens,
+                                    (cudaStream_t)stream);
+  const int f = finish_launches(1, -1);
+  return r != FPB_OK ? r : f;
+}
+
+int fpb_token_scores_bwd(int64_t rows, int32_t V, int32_t dtype, int32_t top, const void* logits, int64_t row_stride, const int64_t* tokens,
+                         const float* entropy, const float* stats, const int64_t* top_tokens, const float* d_logprob, const float* d_entropy,
+                         const float* d_top_logprob, void* d_logits, int64_t d_stride, fpb_stream_t stream) {
+  FPB_TRY(check_scores(rows, V, dtype, top, logits, row_stride, tokens));
+  FPB_TRY(check_scores(rows, V, dtype, top, d_logits, d_stride, tokens));
+  if (rows > 0 && (!entropy || !stats || (d_top_logprob && top > 0 && !top_tokens))) return FPB_ERR_NULL_POINTER;
+  if ((uintptr_t)stats % 8) return FPB_ERR_BAD_STRIDE;
+  FPB_TRY(check_device());
+  if (rows == 0) return FPB_OK;
+  const int r = launch_token_scores_grad(dtype, rows, V, top, logits, row_stride, tokens, entropy, stats, top_tokens, d_logprob, d_entropy,
+                                         top > 0 ? d_top_logprob : nullptr, d_logits, d_stride, (cudaStream_t)stream);
+  const int f = finish_launches(1, -1);
+  return r != FPB_OK ? r : f;
+}
+
 const char* fpb_strerror(int status) {
   switch (status) {
     case FPB_OK: return "ok";

@@ -105,6 +105,29 @@ int launch_xent_fwd(int dtype, int64_t rows, int V, const void* logits, int64_t 
 int launch_xent_bwd(int dtype, int64_t rows, int V, const void* logits, int64_t row_stride, const int64_t* targets, const float* lse,
                     const float* scale, float row_weight, void* d_logits, int64_t d_stride, cudaStream_t stream);
 
+// Norms of queries and keys with the rotation (qk_norm_rotary.cu); backward: `dy`, the weights' gradients `dw` (each may be null)
+// and `partial`, FPB_QK_NORM_SCRATCH(d) bytes.
+int launch_qk_norm(int dtype, bool backward, int B, int T, int Hq, int Hk, int d, float eps, const float* const w[2], const float* phasors,
+                   int64_t phasor_stride_b, const SeqView x[2], const SeqView dy[2], const SeqView out[2], float* const dw[2], float* partial,
+                   cudaStream_t stream);
+
+// Dropout from a counter-based generator (dropout.cu).
+int launch_dropout(int dtype, int64_t n, double prob, const int64_t* seed, const void* x, const void* residual, void* y, cudaStream_t stream);
+
+// Embedding lookup and the table's gradient (embedding.cu).
+int launch_embedding(int dtype, int64_t N, int64_t V, int D, const int64_t* tokens, const void* weight, int64_t w_stride, float scale, void* y,
+                     cudaStream_t stream);
+int64_t embedding_workspace(int64_t N, int64_t V, int D);
+int launch_embedding_grad(int dtype, int64_t N, int64_t V, int D, const int64_t* tokens, int64_t padding, float scale, const void* dy,
+                          int64_t dy_stride, void* dw, void* workspace, cudaStream_t stream, int* n_launched);
+
+// Log probabilities, entropies and alternatives of rows of logits, and their gradient (token_scores.cu).
+int launch_token_scores(int dtype, int64_t rows, int V, int top, const void* logits, int64_t row_stride, const int64_t* tokens, float* logprob,
+                        float* entropy, float* stats, float* top_logprob, int64_t* top_tokens, cudaStream_t stream);
+int launch_token_scores_grad(int dtype, int64_t rows, int V, int top, const void* logits, int64_t row_stride, const int64_t* tokens,
+                             const float* entropy, const float* stats, const int64_t* top_tokens, const float* g_logprob,
+                             const float* g_entropy, const float* g_top, void* d_logits, int64_t d_stride, cudaStream_t stream);
+
 // Per-launch knobs of the tcgen05 kernels.  A release build always passes the defaults; the diagnostics build
 // (-DFPB_DIAGNOSTICS) exports setters so that tests can shorten the wait limit or compare schedules.
 struct WalkTuning {

@@ -1,6 +1,7 @@
 """The elementwise passes of a retention layer either side of the operator, fused: the rotary rotation of q and k
-(flash_pop/xpos_emb.py:32-40,120-126) and GroupNorm-per-head times the swish gate (flash_pop/retnet.py:294-309).
-Each is one streaming CUDA kernel forward and one backward, over the C ABI (fpb_rotary, fpb_groupnorm_gate_*)."""
+(flash_pop/xpos_emb.py:32-40,120-126), with or without norms of their heads before it, GroupNorm-per-head times the swish gate
+(flash_pop/retnet.py:294-309) and dropout added to the residual.  Each is one streaming CUDA kernel forward and one backward, over
+the C ABI (fpb_rotary, fpb_qk_norm_rotary_*, fpb_groupnorm_gate_*, fpb_dropout)."""
 from __future__ import annotations
 
 import ctypes
@@ -8,6 +9,7 @@ from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from flash_pop_b200 import _lib
 
@@ -68,6 +70,150 @@ class RotaryQK(torch.autograd.Function):
 def rotary_qk(q: Tensor, k: Tensor, phasors: Tensor, out_dtype: Optional[torch.dtype] = None) -> Tuple[Tensor, Tensor]:
     """Rotate the channel pairs of q and k (B,T,H,d) by `phasors` (1 or B, T, d/2, 2) = (cos, sin), fp32."""
     return RotaryQK.apply(q, k, phasors, out_dtype)
+
+
+# ---- norms of queries and keys, then the rotation ------------------------------------------------------------------
+def _check_qk_norm(q: Tensor, k: Tensor, q_weight: Optional[Tensor], k_weight: Optional[Tensor], phasors: Optional[Tensor]) -> None:
+    _lib.require_cuda(q, k, q_weight, k_weight, phasors)
+    if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.size(3) != k.size(3):
+        raise ValueError(f"q and k: (B, T, heads, d) with the same B, T and d; got {tuple(q.shape)} and {tuple(k.shape)}")
+    d = q.size(3)
+    if d % 8 or not 0 < d <= 256:
+        raise ValueError(f"the head dimension has to be a multiple of 8 and at most 256; got {d}")
+    if q.dtype not in _OK_DTYPES or k.dtype != q.dtype:
+        raise ValueError(f"q and k: both bfloat16 or both float32; got {q.dtype} and {k.dtype}")
+    for w in (q_weight, k_weight):
+        if w is not None and (w.shape != (d,) or not w.is_floating_point()):
+            raise ValueError(f"the weights have to be floating-point tensors of {d} elements")
+    if phasors is not None and (phasors.dtype != torch.float32 or phasors.dim() != 4 or phasors.size(0) not in (1, q.size(0))
+                                or tuple(phasors.shape[1:]) != (q.size(1), d // 2, 2)):
+        raise ValueError(f"phasors: float32 (1 or {q.size(0)}, {q.size(1)}, {d // 2}, 2); got {phasors.dtype} {tuple(phasors.shape)}")
+    if any(t is not None and t.device != q.device for t in (k, q_weight, k_weight, phasors)):
+        raise ValueError("q, k, the weights and the phasors have to be on one device")
+
+
+class QKNormRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, phasors, eps):
+        q, k = _aligned(q, 16), _aligned(k, 16)
+        B, T, Hq, d = q.shape
+        Hk = k.size(2)
+        y_q, y_k = torch.empty((B, T, Hq, d), device=q.device, dtype=q.dtype), torch.empty((B, T, Hk, d), device=q.device, dtype=q.dtype)
+        step = 0 if phasors is None or phasors.size(0) == 1 else T * (d // 2)
+        with torch.cuda.device(q.device):
+            _lib.check(_lib.lib().fpb_qk_norm_rotary_fwd(B, T, Hq, Hk, d, _lib.dtype_code(q), eps, _ptr(q_weight), _ptr(k_weight), _ptr(phasors),
+                                                         step, _lib.seq(q), _lib.seq(k), _lib.seq(y_q), _lib.seq(y_k), _lib.stream_ptr(q.device)))
+        ctx.save_for_backward(q, k, q_weight, k_weight, phasors)
+        ctx.eps, ctx.step = eps, step
+        return y_q, y_k
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dyq, dyk):
+        q, k, q_weight, k_weight, phasors = ctx.saved_tensors
+        B, T, Hq, d = q.shape
+        Hk = k.size(2)
+        dyq, dyk = _aligned(dyq.to(q.dtype), 16), _aligned(dyk.to(q.dtype), 16)
+        dq, dk = torch.empty((B, T, Hq, d), device=q.device, dtype=q.dtype), torch.empty((B, T, Hk, d), device=q.device, dtype=q.dtype)
+        dwq, dwk = (torch.empty(d, device=q.device, dtype=torch.float32) if n else None for n in ctx.needs_input_grad[2:4])
+        with torch.cuda.device(q.device):
+            scratch = torch.empty(_lib.QK_NORM_SLABS * 2 * d, device=q.device, dtype=torch.float32)
+            _lib.check(_lib.lib().fpb_qk_norm_rotary_bwd(B, T, Hq, Hk, d, _lib.dtype_code(q), ctx.eps, _ptr(q_weight), _ptr(k_weight),
+                                                         _ptr(phasors), ctx.step, _lib.seq(q), _lib.seq(k), _lib.seq(dyq), _lib.seq(dyk),
+                                                         _lib.seq(dq), _lib.seq(dk), _ptr(dwq), _ptr(dwk), _ptr(scratch),
+                                                         _lib.stream_ptr(q.device)))
+        return dq, dk, dwq, dwk, None, None
+
+
+def _norm_weight(w: Optional[Tensor]) -> Optional[Tensor]:
+    if w is None:
+        return None
+    w = w.to(torch.float32).contiguous()
+    return w if w.data_ptr() % 16 == 0 else w.clone()
+
+
+def qk_norm_rotary(q: Tensor, k: Tensor, q_weight: Optional[Tensor], k_weight: Optional[Tensor], phasors: Optional[Tensor],
+                   eps: float = 1e-6) -> Tuple[Tensor, Tensor]:
+    """RMS norm of every head of q (B, T, Hq, d) and k (B, T, Hk, d), ``x / sqrt(mean(x^2) + eps) * weight``, then the rotation of
+    the channel pairs by `phasors` (1 or B, T, d/2, 2) = (cos, sin), fp32 (None: no rotation), in one pass.  The weights
+    (d elements each, None: ones) are shared by the heads; d a multiple of 8, at most 256.  fp32 arithmetic, results in q's dtype.
+    No gradient goes to the phasors; the weights' gradients are summed in a fixed order."""
+    _check_qk_norm(q, k, q_weight, k_weight, phasors)
+    if phasors is not None:
+        phasors = phasors.detach().contiguous()
+        if phasors.data_ptr() % 16:
+            phasors = phasors.clone()
+    return QKNormRotary.apply(q, k, _norm_weight(q_weight), _norm_weight(k_weight), phasors, float(eps))
+
+
+# ---- dropout without a stored mask ------------------------------------------------------------------------------------
+def _flat(t: Tensor) -> Tensor:
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _drop(x: Tensor, p: float, seed: Tensor, residual: Optional[Tensor]) -> Tensor:
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    with torch.cuda.device(x.device):
+        _lib.check(_lib.lib().fpb_dropout(x.numel(), _lib.dtype_code(x), p, _ptr(seed), _ptr(x), _ptr(residual), _ptr(y),
+                                          _lib.stream_ptr(x.device)))
+    return y
+
+
+class Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, p, seed):
+        ctx.save_for_backward(seed)
+        ctx.p = p
+        return _drop(_flat(x), p, seed, None if residual is None else _flat(residual))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        (seed,) = ctx.saved_tensors
+        return _drop(_flat(dy), ctx.p, seed, None) if ctx.needs_input_grad[0] else None, dy if ctx.needs_input_grad[1] else None, None, None
+
+
+def dropout(x: Tensor, p: float, seed: Tensor, residual: Optional[Tensor] = None) -> Tensor:
+    """``residual + x * mask / (1 - p)`` (without a residual: ``x * mask / (1 - p)``) where the mask is a function of `seed`, one
+    int64 on x's device, and of the element's place alone: no mask is stored, and a captured graph draws another one when the seed's
+    content changes.  p counts in steps of 2^-16; what is dropped is 0 whatever it was.  The seed must keep its content until the
+    backward has run."""
+    _lib.require_cuda(x, seed, residual)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"p has to be a probability; got {p}")
+    if x.dtype not in _OK_DTYPES:
+        raise ValueError(f"x: bfloat16 or float32; got {x.dtype}")
+    if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != x.device:
+        raise ValueError("seed: one int64 on the device of x")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+        raise ValueError("the residual has to be of x's shape, type and device")
+    return Dropout.apply(x, residual, float(p), seed)
+
+
+class CounterDropout(torch.nn.Module):
+    """``nn.Dropout`` on `dropout`: a seed from torch's generator for every call, no mask in memory, and the addition of a
+    residual in the same pass.  Reproducible by ``torch.manual_seed`` (other masks than nn.Dropout's), under checkpointing and
+    in captured graphs, as far as torch's generator is."""
+
+    def __init__(self, p: float = 0.5):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"p has to be a probability; got {p}")
+        self.p = p
+
+    def extra_repr(self) -> str:
+        return f"p={self.p}"
+
+    def active(self) -> bool:
+        return self.training and self.p > 0
+
+    def forward(self, x: Tensor, residual: Optional[Tensor] = None) -> Tensor:
+        if not self.active():
+            return x if residual is None else residual + x
+        seed = torch.empty(1, dtype=torch.int64, device=x.device).random_()
+        if residual is not None and (residual.dtype != x.dtype or residual.shape != x.shape):
+            return residual + dropout(x, self.p, seed)
+        return dropout(x, self.p, seed, residual)
 
 
 def groupnorm_gate_supported(o: Tensor, z: Tensor) -> bool:

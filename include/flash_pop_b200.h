@@ -332,6 +332,63 @@ int fpb_cross_entropy_bwd(int64_t rows, int32_t V, int32_t dtype, const void* lo
                           const int64_t* targets, const float* lse, const float* scale, float row_weight,
                           void* d_logits, int64_t d_stride, fpb_stream_t stream);
 
+/*
+ * Norms of queries and keys over each head, then the position rotation, in one pass over (B, T, Hq, d) queries and (B, T, Hk, d)
+ * keys (d a multiple of 8, at most 256; bf16 or fp32, fp32 arithmetic; tensors and strides 16-byte aligned):
+ *   y = R (x r w),  r = 1 / sqrt(mean over d of x^2 + eps)
+ * w_q, w_k: d fp32 weights each, 16-byte aligned, NULL: ones.  phasors as fpb_rotary takes them, NULL: no rotation.
+ * The backward reads x and d_y, writes d_x and, where d_w_q / d_w_k are given (fp32), the weights' gradients: sums over all rows in a
+ * fixed order.  `scratch`: FPB_QK_NORM_SCRATCH(d) device bytes, 16-byte aligned, used during the call only.  The reference
+ * rotates without norms (flash_pop/xpos_emb.py:120-126); the norms are an addition.
+ */
+#define FPB_QK_NORM_SLABS 592
+#define FPB_QK_NORM_SCRATCH(d) ((int64_t)FPB_QK_NORM_SLABS * 2 * (d) * 4)
+int fpb_qk_norm_rotary_fwd(int32_t B, int32_t T, int32_t Hq, int32_t Hk, int32_t d, int32_t dtype, float eps, const float* w_q,
+                           const float* w_k, const float* phasors, int64_t phasor_stride_b, const fpb_seq* q, const fpb_seq* k,
+                           const fpb_seq* q_out, const fpb_seq* k_out, fpb_stream_t stream);
+int fpb_qk_norm_rotary_bwd(int32_t B, int32_t T, int32_t Hq, int32_t Hk, int32_t d, int32_t dtype, float eps, const float* w_q,
+                           const float* w_k, const float* phasors, int64_t phasor_stride_b, const fpb_seq* q, const fpb_seq* k,
+                           const fpb_seq* d_yq, const fpb_seq* d_yk, const fpb_seq* d_q, const fpb_seq* d_k, float* d_w_q, float* d_w_k,
+                           void* scratch, fpb_stream_t stream);
+
+/*
+ * Dropout without a stored mask: y = [residual +] keep ? x / (1 - p) : 0 over n contiguous elements (residual NULL: none; y may
+ * be x).  Element i is kept where its 16 bits, half word i % 8 of Philox4x32-10 of the counter i / 8 under the key *seed, are
+ * at least p in units of 2^-16; the scale is that of the rounded p.  `seed`: one int64 on the device, read by the kernel, so a
+ * captured graph takes a new one at every replay.  The backward is the same call on d_y without a residual.  (The reference
+ * drops with nn.Dropout, flash_pop/retnet.py:452-486.)
+ */
+int fpb_dropout(int64_t n, int32_t dtype, double p, const int64_t* seed, const void* x, const void* residual, void* y, fpb_stream_t stream);
+
+/*
+ * y[n] = scale * weight[tokens[n]] for N ids and a (V, D) table with rows `w_stride` elements apart; y (N, D) contiguous.  An id
+ * outside [0, V) gives a zero row.  The backward writes the whole dense gradient d_weight (V, D), contiguous:
+ *   d_weight[v] = scale * sum of d_y[n] over the n with tokens[n] == v, in the order of n
+ * with fp32 sums, rounded once; ids outside the table and `padding` (-1: none) have no part.  The same bits every time.
+ * `workspace`: fpb_embedding_workspace bytes, 16-byte aligned, used during the call only.
+ */
+int fpb_embedding_fwd(int64_t N, int64_t V, int32_t D, int32_t dtype, const int64_t* tokens, const void* weight, int64_t w_stride,
+                      float scale, void* y, fpb_stream_t stream);
+int64_t fpb_embedding_workspace(int64_t N, int64_t V, int32_t D);
+int fpb_embedding_bwd(int64_t N, int64_t V, int32_t D, int32_t dtype, const int64_t* tokens, int64_t padding, float scale, const void* d_y,
+                      int64_t dy_stride, void* d_weight, void* workspace, int64_t workspace_bytes, fpb_stream_t stream);
+
+/*
+ * Per row of V logits (bf16 or fp32, rows `row_stride` elements apart, no alignment needed), fp32 arithmetic: the log
+ * probability of tokens[row] (0 for one outside [0, V), cross entropy's rule), the entropy of the row, and its `top` (0 to 32, at
+ * most V) most likely tokens with their log probabilities, the most likely first, equal logits by index, NaN before all.
+ * stats: (rows, 2) floats that the backward reads.  A row of -inf only gives log probabilities of -inf and entropy 0; NaN or +inf
+ * in a row make its numbers NaN.
+ * The backward writes the gradient of the logits, in their type, from those of the three results (each may be NULL): every
+ * element of the row, rows `d_stride` apart, zero for a row of -inf only.  `entropy`, `stats` and `top_tokens` are the forward's.
+ */
+#define FPB_MAX_TOP 32
+int fpb_token_scores_fwd(int64_t rows, int32_t V, int32_t dtype, int32_t top, const void* logits, int64_t row_stride, const int64_t* tokens,
+                         float* logprob, float* entropy, float* stats, float* top_logprob, int64_t* top_tokens, fpb_stream_t stream);
+int fpb_token_scores_bwd(int64_t rows, int32_t V, int32_t dtype, int32_t top, const void* logits, int64_t row_stride, const int64_t* tokens,
+                         const float* entropy, const float* stats, const int64_t* top_tokens, const float* d_logprob, const float* d_entropy,
+                         const float* d_top_logprob, void* d_logits, int64_t d_stride, fpb_stream_t stream);
+
 /* Text for a status code. */
 const char* fpb_strerror(int status);
 /* Library version, major*10000 + minor*100 + patch. */
