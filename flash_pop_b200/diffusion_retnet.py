@@ -11,6 +11,7 @@ import torch
 import torch.nn as nn
 from torch import Tensor
 
+from flash_pop_b200.layer_ops import CounterDropout
 from flash_pop_b200.modules.adaln import AdaLayerNorm, AdaLayerNormZero, _to_tokens, gated_residual
 from flash_pop_b200.recurrent_state import RecurrentState
 from flash_pop_b200.retnet import ActivationString, MultiScaleRetention, RetNetDecoder, _get_activation_fn
@@ -34,12 +35,15 @@ class DiffusionRetNetDecoderLayer(nn.Module):
         dtype: Optional[torch.dtype] = torch.bfloat16
         use_fused_version: bool = True
         chunk_size: int = 512  # accepted for compatibility; unused
+        qk_norm: bool = False          # RMS norm of every head of q and k before the rotation, weights shared by the heads
+        qk_norm_eps: float = 1e-6
+        counter_dropout: bool = False  # dropout without a stored mask (other masks than torch's for the same seed)
 
     def __init__(self, config: Config, xpos_embedder: Optional[XPos] = None) -> None:
         super().__init__()
         self.config = config
         self.activation = _get_activation_fn(config.activation) if isinstance(config.activation, str) else config.activation
-        self.dropout = nn.Dropout(config.dropout)
+        self.dropout = CounterDropout(config.dropout) if config.counter_dropout else nn.Dropout(config.dropout)
         self.use_post_retention_dropout = config.use_post_retention_dropout
         d_model = config.num_heads * config.head_dim_v
         ada = dict(eps=config.layer_norm_eps, lora_hidden_dim=config.ada_ln_lora_dim, device=config.device, dtype=config.dtype)
@@ -55,7 +59,8 @@ class DiffusionRetNetDecoderLayer(nn.Module):
         return MultiScaleRetention(MultiScaleRetention.Config(
             num_heads=c.num_heads, head_dim_v=c.head_dim_v, head_dim_qk=c.head_dim_qk, dropout=c.dropout,
             head_decays_range=c.head_decays_range, activation=self.activation, device=c.device, dtype=c.dtype,
-            use_fused_version=c.use_fused_version, chunk_size=c.chunk_size), xpos_embedder=xpos_embedder)
+            use_fused_version=c.use_fused_version, chunk_size=c.chunk_size, qk_norm=c.qk_norm, qk_norm_eps=c.qk_norm_eps,
+            counter_dropout=c.counter_dropout), xpos_embedder=xpos_embedder)
 
     def _reset_parameters(self):
         for lin in (self.linear1, self.linear2):
@@ -72,7 +77,8 @@ class DiffusionRetNetDecoderLayer(nn.Module):
         x, gate = self.ada_ln1.forward_rows(x, c)
         y, state = retention_fn(x)
         if self.use_post_retention_dropout and self.training and self.dropout.p > 0:
-            x = x + self.dropout(y * _to_tokens(gate, x.size(1)))
+            y = y * _to_tokens(gate, x.size(1))
+            x = self.dropout(y, x) if type(self.dropout) is CounterDropout else x + self.dropout(y)
         else:
             x = gated_residual(x, y, gate)
         x, gate = self.ada_ln2.forward_rows(x, c)

@@ -26,7 +26,8 @@ import torch.nn.functional as F
 from torch import Tensor
 
 from flash_pop_b200.fused_retention import cuda_core_kernels, fused_chunk_retention, retention_step
-from flash_pop_b200.layer_ops import SwishFeedForward, groupnorm_gate, groupnorm_gate_supported, linear_group, linears_supported, norm_in_fp32
+from flash_pop_b200.layer_ops import (CounterDropout, SwishFeedForward, groupnorm_gate, groupnorm_gate_supported, linear_group, linears_supported,
+                                      norm_in_fp32, qk_norm_rotary)
 from flash_pop_b200.recurrent_state import RecurrentState
 from flash_pop_b200.token_stack import decoder_token
 from flash_pop_b200.xpos_emb import XPos
@@ -99,6 +100,9 @@ class MultiScaleRetention(nn.Module):
         dtype: Optional[torch.dtype] = torch.bfloat16
         use_fused_version: bool = True
         chunk_size: int = 512  # accepted for compatibility; unused
+        qk_norm: bool = False          # RMS norm of every head of q and k before the rotation, weights shared by the heads
+        qk_norm_eps: float = 1e-6
+        counter_dropout: bool = False  # dropout without a stored mask (other masks than torch's for the same seed)
 
     def __init__(self, config: Config, xpos_embedder: Optional[XPos] = None):
         super().__init__()
@@ -110,6 +114,7 @@ class MultiScaleRetention(nn.Module):
         if self.head_dim_v % 8 != 0:
             raise ValueError(f"head_dim (embed_dim / num_heads = {self.head_dim_v}) must be divisible by 8")
         self.dropout = config.dropout
+        self.drop = CounterDropout(config.dropout) if config.counter_dropout else None
         self.relative_position = config.relative_position
         self.bias = config.bias
         self.activation = _get_activation_fn(config.activation) if isinstance(config.activation, str) else config.activation
@@ -129,6 +134,12 @@ class MultiScaleRetention(nn.Module):
                                        eps=config.group_norm_eps, device=config.device, dtype=torch.float32)
         self.g_proj = nn.Linear(embed_dim, embed_dim, **kw)
         self.out_proj = nn.Linear(embed_dim, embed_dim, **kw)
+        self.qk_norm = config.qk_norm
+        if config.qk_norm:
+            if self.head_dim_qk % 8 or self.head_dim_qk > 256:
+                raise ValueError(f"qk_norm needs a head dimension of q and k that is a multiple of 8 and at most 256; got {self.head_dim_qk}")
+            self.q_norm_weight = nn.Parameter(torch.ones(self.head_dim_qk, device=config.device, dtype=torch.float32))
+            self.k_norm_weight = nn.Parameter(torch.ones(self.head_dim_qk, device=config.device, dtype=torch.float32))
         self._reset_parameters()
 
     def _reset_parameters(self):
@@ -159,9 +170,13 @@ class MultiScaleRetention(nn.Module):
                 gated = groupnorm_gate(o4, z4 if swish else self.activation(z4), self.group_norm.eps, swish)
                 return linear_group(gated.reshape(*shape, self.embed_dim), self.out_proj)[0]
         flat = retention.reshape(-1, self.embed_dim)
-        flat = F.dropout(flat, p=self.dropout, training=self.training)
+        flat = F.dropout(flat, p=self.dropout, training=self.training) if self.drop is None else self.drop(flat)
         flat = self.group_norm(flat.float()).to(dtype=x.dtype)
         return self.out_proj(flat.view(*shape, self.embed_dim) * self.activation(z))
+
+    def _norm_and_rotate(self, q: Tensor, k: Tensor, start_idx: Union[int, torch.LongTensor], xpos: XPos) -> Tuple[Tensor, Tensor]:
+        phasors = xpos.phasors(q, start_idx) if self.relative_position else None
+        return qk_norm_rotary(q, k, self.q_norm_weight, self.k_norm_weight, phasors, self.config.qk_norm_eps)
 
     def _retention_chunkwise(self, x: Tensor, start_idx: Union[int, torch.LongTensor], prev_state: Optional[Tensor] = None,
                              retention_kernel: Optional[Callable] = None, xpos_embedder: Optional[XPos] = None):
@@ -172,7 +187,9 @@ class MultiScaleRetention(nn.Module):
         else:
             q, k, v = linear_group(x, self.q_proj, self.k_proj, self.v_proj)
         q, k, v = (_split_heads(t.to(dtype=x.dtype), self.num_heads) for t in (q, k, v))
-        if self.relative_position:
+        if self.qk_norm:
+            q, k = self._norm_and_rotate(q, k, start_idx, xpos_embedder or self.xpos_embedder)
+        elif self.relative_position:
             q, k = (xpos_embedder or self.xpos_embedder)(q, k, start_idx)
         if prev_state is None:
             prev_state = torch.zeros((x.size(0), self.num_heads, self.head_dim_qk, self.head_dim_v), device=x.device, dtype=x.dtype)
@@ -189,7 +206,9 @@ class MultiScaleRetention(nn.Module):
         q = _split_heads(self.q_proj(x), self.num_heads)
         k = _split_heads(self.k_proj(x), self.num_heads)
         v = _split_heads(self.v_proj(x), self.num_heads)
-        if self.relative_position:
+        if self.qk_norm:
+            q, k = (t.squeeze(1) for t in self._norm_and_rotate(q.unsqueeze(1), k.unsqueeze(1), seq_idx, self.xpos_embedder))
+        elif self.relative_position:
             q, k = self.xpos_embedder(q, k, seq_idx)
         retention, state = retention_recurrent(q, k, v, self.head_decays_torch.to(x.device), prev_state=prev_state,
                                                decays=self.head_decays)
@@ -215,12 +234,15 @@ class RetNetDecoderLayer(nn.Module):
         dtype: Optional[torch.dtype] = torch.bfloat16
         use_fused_version: bool = True
         chunk_size: int = 512  # accepted for compatibility; unused
+        qk_norm: bool = False          # RMS norm of every head of q and k before the rotation, weights shared by the heads
+        qk_norm_eps: float = 1e-6
+        counter_dropout: bool = False  # dropout without a stored mask, added to the residual in one pass (other masks than torch's)
 
     def __init__(self, config: Config, xpos_embedder: Optional[XPos] = None) -> None:
         super().__init__()
         self.config = config
         self.activation = _get_activation_fn(config.activation) if isinstance(config.activation, str) else config.activation
-        self.dropout = nn.Dropout(config.dropout)
+        self.dropout = CounterDropout(config.dropout) if config.counter_dropout else nn.Dropout(config.dropout)
         self.norm_first = config.norm_first
         d_model = config.num_heads * config.head_dim_v
         ln = dict(eps=config.layer_norm_eps, device=config.device, dtype=torch.float32)   # fp32 norms, as the reference
@@ -234,7 +256,8 @@ class RetNetDecoderLayer(nn.Module):
     def _retention_config_kwargs(self) -> dict:
         c = self.config
         return dict(num_heads=c.num_heads, head_dim_v=c.head_dim_v, head_dim_qk=c.head_dim_qk, dropout=c.dropout,
-                    head_decays_range=c.head_decays_range, activation=self.activation, device=c.device, dtype=c.dtype)
+                    head_decays_range=c.head_decays_range, activation=self.activation, device=c.device, dtype=c.dtype,
+                    qk_norm=c.qk_norm, qk_norm_eps=c.qk_norm_eps, counter_dropout=c.counter_dropout)
 
     def _build_multi_scale_retention(self, xpos_embedder: Optional[XPos] = None):
         cfg = MultiScaleRetention.Config(use_fused_version=self.config.use_fused_version, chunk_size=self.config.chunk_size,
@@ -248,20 +271,30 @@ class RetNetDecoderLayer(nn.Module):
 
     def _feedforward_block(self, x: Tensor) -> Tensor:
         drop = self.dropout
-        if (self.activation is F.silu and type(drop) is nn.Dropout and (drop.p == 0 or not drop.training) and not drop._forward_hooks
+        if (self.activation is F.silu and type(drop) in (nn.Dropout, CounterDropout) and (drop.p == 0 or not drop.training) and not drop._forward_hooks
                 and not drop._forward_pre_hooks and linears_supported(x, self.linear1, self.linear2)):
             return SwishFeedForward.apply(x, self.linear1.weight, self.linear1.bias, self.linear2.weight, self.linear2.bias)
         x = self.dropout(self.activation(self.linear1(x)))
         return self.dropout(self.linear2(x))
 
-    def _residual_blocks(self, x: Tensor, retention_fn: Callable[[Tensor], Tuple[Tensor, Tensor]], fp32_norm: bool):
-        """x + retention, x + feed-forward, with the norm before (pre-norm) or after each branch."""
+    def _adds_dropout(self) -> bool:
+        """Whether what a branch drops is added to the residual in the same pass."""
+        return (self.norm_first and type(self.dropout) is CounterDropout and self.dropout.active()
+                and type(self)._residual_blocks is RetNetDecoderLayer._residual_blocks)
+
+    def _residual_blocks(self, x: Tensor, retention_fn: Callable[[Tensor], Tuple[Tensor, Tensor]], fp32_norm: bool, drop: bool = False):
+        """x + retention, x + feed-forward, with the norm before (pre-norm) or after each branch.  `drop`: the retention still has
+        to go through the dropout."""
         dtype = self.config.dtype
         norm = (lambda m, t: norm_in_fp32(m, t).to(dtype=dtype)) if fp32_norm else (lambda m, t: m(t))
         if self.norm_first:
             y, state = retention_fn(norm(self.norm1, x))
-            x = x + y
-            x = x + self._feedforward_block(norm(self.norm2, x))
+            x = self.dropout(y, x) if drop else x + y
+            h = norm(self.norm2, x)
+            if self._adds_dropout() and type(self)._feedforward_block is RetNetDecoderLayer._feedforward_block:
+                x = self.dropout(self.linear2(self.dropout(self.activation(self.linear1(h)))), x)
+            else:
+                x = x + self._feedforward_block(h)
         else:
             y, state = retention_fn(x)
             x = x + norm(self.norm1, y)
@@ -269,10 +302,12 @@ class RetNetDecoderLayer(nn.Module):
         return x, state
 
     def forward_chunkwise(self, x: Tensor, start_idx: int, prev_state: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+        later = self.config.use_post_retention_dropout and self._adds_dropout()
+
         def branch(h):
             y, state = self.retention.forward_chunkwise(h, start_idx=start_idx, prev_state=prev_state)
-            return (self.dropout(y) if self.config.use_post_retention_dropout else y), state
-        return self._residual_blocks(x, branch, fp32_norm=True)
+            return (self.dropout(y) if self.config.use_post_retention_dropout and not later else y), state
+        return self._residual_blocks(x, branch, fp32_norm=True, **({"drop": True} if later else {}))
 
     def forward_recurrent(self, x: Tensor, seq_idx: int, prev_state: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
         def branch(h):

@@ -13,15 +13,21 @@ import torch.nn.functional as F
 from flash_pop_b200.layer_ops import norm_in_fp32
 from flash_pop_b200.recurrent_state import RecurrentState
 from flash_pop_b200.retnet import RetNetDecoder, RetNetDecoderLayer
+from flash_pop_b200.token_ops import TokenScores, embedding, token_scores
 
 
 class RetNetLM(nn.Module):
     def __init__(self, vocab_size: int = 32000, num_layers: int = 12, num_heads: int = 8, head_dim: int = 128,
-                 dim_feedforward: int = 4096, dropout: float = 0.0, device="cuda", dtype=torch.bfloat16):
+                 dim_feedforward: int = 4096, dropout: float = 0.0, device="cuda", dtype=torch.bfloat16, embed_scale: Optional[float] = None,
+                 qk_norm: bool = False, counter_dropout: bool = False):
+        """embed_scale: the embedding's rows are multiplied by it, and its gradient is summed in a fixed order (None: a plain
+        ``nn.Embedding``).  qk_norm, counter_dropout: see RetNetDecoderLayer.Config."""
         super().__init__()
         d_model = num_heads * head_dim
         cfg = RetNetDecoderLayer.Config(num_heads=num_heads, head_dim_v=head_dim, head_dim_qk=head_dim,
-                                        dim_feedforward=dim_feedforward, dropout=dropout, device=device, dtype=dtype)
+                                        dim_feedforward=dim_feedforward, dropout=dropout, device=device, dtype=dtype, qk_norm=qk_norm,
+                                        counter_dropout=counter_dropout)
+        self.embed_scale = embed_scale
         self.embed = nn.Embedding(vocab_size, d_model, device=device, dtype=dtype)
         self.decoder = RetNetDecoder(cfg, num_layers)
         self.norm = nn.LayerNorm(d_model, device=device, dtype=torch.float32)
@@ -31,13 +37,21 @@ class RetNetLM(nn.Module):
 
     def forward(self, tokens: torch.Tensor, recurrent_state: Optional[RecurrentState] = None):
         """tokens: (B, T) int64 -> logits (B, T, vocab), new RecurrentState."""
-        x, state = self.decoder(self.embed(tokens), recurrent_state)
+        x = self.embed(tokens) if self.embed_scale is None else embedding(tokens, self.embed.weight, self.embed_scale)
+        x, state = self.decoder(x, recurrent_state)
         return self.head(norm_in_fp32(self.norm, x)), state
 
     def loss(self, tokens: torch.Tensor) -> torch.Tensor:
         """Next-token cross entropy of `tokens` (B, T)."""
         logits, _ = self(tokens[:, :-1])
         return F.cross_entropy(logits.float().flatten(0, 1), tokens[:, 1:].flatten())
+
+    def score(self, tokens: torch.Tensor, top: int = 0) -> TokenScores:
+        """What the model says of `tokens` (B, T): for each of positions 1 to T-1 the log probability of the token that stands there,
+        the entropy of the distribution it came from and, with `top`, the most likely tokens with their log probabilities; all
+        (B, T-1[, top]), differentiable."""
+        logits, _ = self(tokens[:, :-1])
+        return token_scores(logits, tokens[:, 1:], top)
 
     def flops_per_token(self, seq_len: int) -> float:
         """Training (forward + backward) FLOPs per token: 6 x matmul parameters + the retention operator."""

@@ -14,7 +14,7 @@ import torch.nn.functional as F
 from torch import Tensor
 
 from flash_pop_b200 import _lib
-from flash_pop_b200.layer_ops import observed, plain_linear
+from flash_pop_b200.layer_ops import CounterDropout, observed, plain_linear
 from flash_pop_b200.recurrent_state import RecurrentState
 from flash_pop_b200.xpos_emb import XPos
 
@@ -79,7 +79,9 @@ def _layer(layer, first, shape, x_device, index, layer_cls, retention_cls, kept:
         return None
     drop = mods["dropout"]
     dd = drop.__dict__
-    if type(drop) is not nn.Dropout or dd["_forward_hooks"] or dd["_forward_pre_hooks"] or (drop.p > 0 and drop.training):
+    if type(drop) not in (nn.Dropout, CounterDropout) or dd["_forward_hooks"] or dd["_forward_pre_hooks"] or (drop.p > 0 and drop.training):
+        return None
+    if rown.get("qk_norm", False):                # (a step the kernels do not have)
         return None
     if (ret.dropout > 0 and ret.training) or (ret.num_heads, ret.head_dim_qk, ret.head_dim_v) != (H, dk, dv) or ret.head_decays != first.head_decays:
         return None

@@ -73,6 +73,11 @@ class XPos:
             ph = ph.reshape(ph.shape[0], 1, -1)
         return torch.view_as_real(xc * ph).flatten(-2).to(x.dtype)
 
+    def phasors(self, q: Tensor, start_idx: Union[int, Tensor]) -> Tensor:
+        """(cos, sin) by which `__call__` rotates q (B, T, H, d): (1 or B, T, d/2, 2) fp32 on its device."""
+        self._move(q.device)
+        return torch.view_as_real(self._rotation(q.size(1), start_idx)).contiguous()
+
     def __call__(self, q: Tensor, k: Tensor, start_idx: Union[int, Tensor], *args, **kwargs):
         self._move(q.device)
         seq_len = q.size(1) if q.dim() == 4 else 1
