@@ -774,7 +774,7 @@ int fpb_dropout(int64_t n, int32_t dtype, double p, const int64_t* seed, const v
 namespace {
 int check_embedding(int64_t N, int64_t V, int32_t D, int32_t dtype, const int64_t* tokens) {
   if (N < 0 || V <= 0 || D <= 0) return FPB_ERR_BAD_SHAPE;
-  if (N >= (1ll << 31) || V >= (1ll << 31)) return FPB_ERR_TOO_LARGE;
+  if (N >= (1ll << 31) || V >= (1ll << 31) || D > (1 << 20)) return FPB_ERR_TOO_LARGE;
   if (!dtype_ok(dtype)) return FPB_ERR_BAD_DTYPE;
   if (N > 0 && !tokens) return FPB_ERR_NULL_POINTER;
   return (uintptr_t)tokens % 8 ? FPB_ERR_BAD_STRIDE : FPB_OK;

@@ -364,7 +364,7 @@ int fpb_dropout(int64_t n, int32_t dtype, double p, const int64_t* seed, const v
  * y[n] = scale * weight[tokens[n]] for N ids and a (V, D) table with rows `w_stride` elements apart; y (N, D) contiguous.  An id
  * outside [0, V) gives a zero row.  The backward writes the whole dense gradient d_weight (V, D), contiguous:
  *   d_weight[v] = scale * sum of d_y[n] over the n with tokens[n] == v, in the order of n
- * with fp32 sums, rounded once; ids outside the table and `padding` (-1: none) have no part.  The same bits every time.
+ * (D at most 2^20) with fp32 sums, rounded once; ids outside the table and `padding` (-1: none) have no part.  The same bits every time.
  * `workspace`: fpb_embedding_workspace bytes, 16-byte aligned, used during the call only.
  */
 int fpb_embedding_fwd(int64_t N, int64_t V, int32_t D, int32_t dtype, const int64_t* tokens, const void* weight, int64_t w_stride,
