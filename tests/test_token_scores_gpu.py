@@ -8,6 +8,10 @@ pytestmark = pytest.mark.gpu
 BF, F32 = torch.bfloat16, torch.float32
 HALF = {BF: 2.0 ** -8, F32: 2.0 ** -24}
 
+# z - m and then - log s round a value of the result's size twice (2^-23 of it).  log s: every exponent is off by 2^-24 of itself
+# (below 100 where it counts), the sums by 2^-24 for each addition of a chain: together below 512 roundings.  H below 128.
+TOL = 512 * 2.0 ** -24
+
 
 def _reference(z, tokens, top):
     """In doubles, row by row rules of the operator included."""
@@ -38,7 +42,8 @@ def _gradient(ref, tokens, g1, g2, g3):
     g1 = torch.where(inside, g1.double(), 0.0)
     total = g1 + (0 if index is None else g3.double().sum(1))
     d = -p * (total[:, None] + g2.double()[:, None] * (torch.where(p == 0, 0.0, logp) + H[:, None]))
-    size = p * (total.abs()[:, None] + (g2.double().abs()[:, None] * (torch.where(p == 0, 0.0, logp).abs() + H[:, None])))
+    # (a p below 2^-126, fp32's smallest normal number, counts as 0: off by less than that, times its factor)
+    size = torch.where(p == 0, 0.0, p + 2.0 ** -126 / (4 * TOL)) * (total.abs()[:, None] + (g2.double().abs()[:, None] * (torch.where(p == 0, 0.0, logp).abs() + H[:, None])))
     d.scatter_add_(1, tokens.clamp(0, d.size(1) - 1)[:, None], g1[:, None])
     size.scatter_add_(1, tokens.clamp(0, d.size(1) - 1)[:, None], g1.abs()[:, None])
     if index is not None:
@@ -52,9 +57,7 @@ def _check(z, tokens, top, grad=True):
     leaf = z.detach().requires_grad_(grad)
     s = token_scores(leaf, tokens, top)
     ref = _reference(z, tokens, top)
-    # z - m and then - log s round a value of the result's size twice (2^-23 of it).  log s: every exponent is off by 2^-24 of itself
-    # (below 100 where it counts), the sums by 2^-24 for each addition of a chain: together below 512 roundings.  H below 128.
-    tol = 512 * 2.0 ** -24
+    tol = TOL
 
     def near(a, b):
         return bool((torch.where(b.isfinite(), (a.double() - b).abs() <= tol + 2.0 ** -22 * b.abs(), (a.double() == b) | (a.isnan() & b.isnan()))).all())
