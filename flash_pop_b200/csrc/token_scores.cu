@@ -7,6 +7,8 @@
 // Bound by HBM: one read forward, one read and one write backward.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "fpb_common.cuh"
 #include "vec_io.cuh"
 
@@ -62,49 +64,35 @@ __device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
 }
 
 // ---- a row as vectors -----------------------------------------------------------------------------------------------
-// A row starts at any element; it is read as the 16-byte vectors that it lies in, the first and the last element by element.
+// A row starts at any element: it is so many single elements up to a 16-byte boundary, whole vectors, and a rest.
 template <int N> struct Vectors {
   uint4 r[N];
 };
 template <typename T> struct Row {
   static constexpr int E = 16 / sizeof(T);
   const T* z;
-  int V, skew, vectors;             // element i is number (i + skew) % E of vector (i + skew) / E
-  int inner, inner_end;             // vectors that lie in the row as a whole
+  int V, head, vectors;
 
   __device__ Row(const void* logits, int64_t row, int64_t stride, int n) : z((const T*)logits + row * stride), V(n) {
-    skew = (int)(((uintptr_t)z % 16) / sizeof(T));
-    vectors = (skew + V + E - 1) / E;
-    inner = skew ? 1 : 0;
-    inner_end = (skew + V) / E;
+    const int skew = (int)(((uintptr_t)z % 16) / sizeof(T));
+    head = min(skew ? E - skew : 0, V);
+    vectors = (V - head) / E;
   }
-  __device__ __forceinline__ int index(int vector, int e) const { return vector * E + e - skew; }
-  __device__ __forceinline__ bool whole(int vector) const { return vector >= inner && vector < inner_end; }
-  __device__ __forceinline__ bool real(int i) const { return (unsigned)i < (unsigned)V; }
-  __device__ __forceinline__ const uint4* base() const { return reinterpret_cast<const uint4*>(z - skew); }
-  // what of a vector is not of the row counts as -inf
-  __device__ __forceinline__ uint4 read(int vector) const { return whole(vector) ? base()[vector] : read_part(z, V, index(vector, 0)); }
-  static __device__ __noinline__ uint4 read_part(const T* z, int V, int first) {
-    uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int i = first + e;
-      const bool real = (unsigned)i < (unsigned)V;
-      if constexpr (sizeof(T) == 2) w[e / 2] |= (real ? (uint32_t)reinterpret_cast<const uint16_t*>(z)[i] : 0xff80u) << (e & 1 ? 16 : 0);
-      else w[e] = real ? reinterpret_cast<const uint32_t*>(z)[i] : 0xff800000u;
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-  }
-  // a thread's vectors first, first + NT, ...; those from `end` on are filled with a value that no sum feels
+  __device__ __forceinline__ int index(int vector, int e) const { return head + vector * E + e; }
+  __device__ __forceinline__ const uint4* base() const { return reinterpret_cast<const uint4*>(z + head); }
+  // the elements outside the vectors, fewer than 2 E
+  __device__ __forceinline__ int edges() const { return V - vectors * E; }
+  __device__ __forceinline__ int edge(int i) const { return i < head ? i : i + vectors * E; }
+  // a thread's vectors tile + its number, and every NT-th after it; those from `end` on are filled with a value that no sum feels
   template <int NT, int N> __device__ __forceinline__ void read(Vectors<N>& to, int tile, int end) const {
-    const int first = tile + threadIdx.x;
-    if (tile >= inner && tile + N * NT <= min(end, inner_end)) {
+    const uint4* from = base() + tile + threadIdx.x;
+    if (tile + N * NT <= end) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) to.r[j] = base()[first + j * NT];
+      for (int j = 0; j < N; ++j) to.r[j] = from[j * NT];
     } else {
-      const uint32_t w = sizeof(T) == 2 ? 0xf149f149u : 0xf149f2cau;          // -1e30
+      const uint32_t w = sizeof(T) == 2 ? 0xf149f149u : 0xf149f2cau;          // FILL and a little
 #pragma unroll
-      for (int j = 0; j < N; ++j) to.r[j] = first + j * NT < end ? read(first + j * NT) : make_uint4(w, w, w, w);
+      for (int j = 0; j < N; ++j) to.r[j] = tile + (int)threadIdx.x + j * NT < end ? from[j * NT] : make_uint4(w, w, w, w);
     }
   }
 };
@@ -129,7 +117,7 @@ template <typename T> __device__ __forceinline__ float largest(const uint4& r) {
 // In powers of two: with L = log2 e and c = m L rounded, x = 2^(z L - c) is one rounding of the exponent (a fused product) and one
 // exponential; that c is not m L exactly shifts all exponents alike and is put right once, in the logarithm of the sum.  Where
 // c could overflow, and where a mask has filled what is left with huge negative numbers, x = 2^((z - m) L).
-constexpr float LARGEST = 2e38f, SMALLEST = -1e29f;
+constexpr float LARGEST = 2e38f, SMALLEST = -1e29f, FILL = -9e29f;
 __device__ __forceinline__ bool ordinary(float m) { return m > SMALLEST && m < LARGEST; }
 __device__ __forceinline__ float origin(float m) { return __fmul_rn(m, LOG2E); }        // c (never fused into what follows)
 __device__ __forceinline__ float exponent(float z, float m) { return ordinary(m) ? fmaf(z, LOG2E, -origin(m)) : (z - m) * LOG2E; }
@@ -181,6 +169,20 @@ template <typename T, int N> __device__ __noinline__ float2 careful_sums(const V
     }
   }
   return make_float2(s, t);
+}
+
+// The largest of a thread's vectors, of which the first `count` are of the row.
+template <typename T, int N> __device__ __forceinline__ float largest_of(const Vectors<N>& from, int count) {
+  float most = largest<T>(from.r[0]);
+#pragma unroll
+  for (int j = 1; j < N; ++j) most = max_nan(most, largest<T>(from.r[j]));
+  if (count < N && !(most > FILL)) {                 // (what stands for those behind the row is more than a mask's value)
+    most = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (j < count) most = max_nan(most, largest<T>(from.r[j]));
+  }
+  return most;
 }
 
 // N vectors of a thread, of which the first `count` are of the row and the first `slots` are of some thread's; most: their largest
@@ -251,18 +253,22 @@ struct ScoreParams {
   int32_t V, top, split;                            // CTAs (of a cluster) that share a row
 };
 
-constexpr int U = 8;                  // vectors of a thread: a tile of the row stays in the CTA's registers
-constexpr int CANDIDATES = 512, MAX_SPLIT = 8, FEW = 20;
+constexpr int N = 4, U = 8;           // vectors of a thread: in flight at a time, and in a tile that is looked at more closely
+constexpr int RECORDS = 512, CANDIDATES = 256, MAX_EDGES = 14, MAX_SPLIT = 8, FEW = 20;
 
 typedef Vectors<U> Tile;
-template <int WARPS> struct Shared {
-  alignas(16) uint64_t candidate[CANDIDATES];       // (both are read two at a time)
-  alignas(16) uint64_t best[MAX_SPLIT * 32];        // the alternatives of a row's CTAs, in the first one
-  uint32_t group[2][64];              // the largest of each part of a tile, tiles in turn
-  int found;
-  uint32_t count[WARPS];
+template <int WARPS> struct Sums {
   Stats parts[WARPS];
-  Stats shares[MAX_SPLIT];            // sums of a row's CTAs, in the first one
+  Stats shares[MAX_SPLIT];            // of a row's CTAs, in the first one
+};
+template <int WARPS> struct Shared {
+  static constexpr int LISTS = WARPS == 8 ? MAX_SPLIT : 1;      // (shorter rows are not shared)
+  alignas(16) uint64_t candidate[CANDIDATES + MAX_EDGES];       // (both are read two at a time)
+  alignas(16) uint64_t best[LISTS * 32];                        // the alternatives of a row's CTAs, in the first one
+  uint2 record[RECORDS];              // order of the largest of a thread's N vectors, the first of them
+  uint32_t group[2][64];              // the largest of each part of a tile, tiles in turn
+  int records, found;
+  uint32_t count[WARPS];
 };
 
 // For each of n keys (unique but for 0, which stands for none) that is among the `top` largest: to(key, how many are larger).
@@ -297,16 +303,13 @@ template <typename T, int NT> __device__ __noinline__ void exact_candidates(cons
     return all;
   };
   auto order = [&](int j, int e) { return order_of(element<T>(r[j], e)) >> SHIFT; };
-  auto here = [&](int j, int e) {
-    const int v = first + j * NT + threadIdx.x;
-    return v < end && row.real(row.index(v, e));
-  };
+  auto here = [&](int j) { return first + j * NT + (int)threadIdx.x < end; };
   auto at_or_above = [&](uint32_t bound) {
     int n = 0;
 #pragma unroll
     for (int j = 0; j < U; ++j)
 #pragma unroll
-      for (int e = 0; e < Row<T>::E; ++e) n += here(j, e) && order(j, e) >= bound;
+      for (int e = 0; e < Row<T>::E; ++e) n += here(j) && order(j, e) >= bound;
     return total(n);
   };
   uint32_t lo = 0, hi = 0xffffffffu >> SHIFT;
@@ -322,7 +325,7 @@ template <typename T, int NT> __device__ __noinline__ void exact_candidates(cons
   for (int j = 0; j < U; ++j)
 #pragma unroll
     for (int e = 0; e < Row<T>::E; ++e)
-      if (here(j, e) && order(j, e) > lo) to[atomicAdd(&sh.found, 1)] = rank_key(element<T>(r[j], e), row.index(first + j * NT + threadIdx.x, e));      // (fewer than top)
+      if (here(j) && order(j, e) > lo) to[atomicAdd(&sh.found, 1)] = rank_key(element<T>(r[j], e), row.index(first + j * NT + threadIdx.x, e));      // (fewer than top)
   __syncthreads();
   int taken = sh.found;
 #pragma unroll
@@ -330,7 +333,7 @@ template <typename T, int NT> __device__ __noinline__ void exact_candidates(cons
     if (taken >= top) break;
     unsigned equal = 0;
 #pragma unroll
-    for (int e = 0; e < Row<T>::E; ++e) equal |= (here(j, e) && order(j, e) == lo ? 1u : 0u) << e;
+    for (int e = 0; e < Row<T>::E; ++e) equal |= (here(j) && order(j, e) == lo ? 1u : 0u) << e;
     int before = __popc(equal);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -354,120 +357,174 @@ template <typename T, int NT> __device__ __noinline__ void exact_candidates(cons
   __syncthreads();
 }
 
+// The largest maxima of the parts that a tile is cut into, sorted, one a lane of every warp: 32 parts, or 64 where more than FEW
+// alternatives are wanted.  `most`: a thread's maximum.  One barrier.
+template <int NT> __device__ __forceinline__ uint32_t part_maxima(float most, bool few, uint32_t (&group)[64]) {
+  const int lane = threadIdx.x & 31;
+  uint32_t g = order_of(most);
+  if (NT == 32) return sort_warp(g);
+#pragma unroll
+  for (int o = 1; o < NT / 64; o *= 2) g = max(g, __shfl_xor_sync(ALL, g, o));
+  if (few) {
+    g = max(g, __shfl_xor_sync(ALL, g, NT / 64));
+    if (lane % (NT / 32) == 0) group[threadIdx.x / (NT / 32)] = g;
+  } else if (lane % (NT / 64 ? NT / 64 : 1) == 0) {
+    group[threadIdx.x / (NT / 64 ? NT / 64 : 1)] = g;
+  }
+  __syncthreads();
+  const uint32_t sorted = sort_warp(group[lane]);
+  return few ? sorted : merge_sorted(sorted, sort_warp(group[32 + lane]));
+}
+
+// The elements of a thread's vectors that reach the bound join the candidates, as far as there is room.
+template <typename T, int NT, int N> __device__ __forceinline__ void push(const Row<T>& row, const Vectors<N>& from, int first, int end, float bound,
+                                                                         Shared<NT / 32>& sh) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int v = first + j * NT + threadIdx.x;
+    if (v >= end || largest<T>(from.r[j]) < bound) continue;
+#pragma unroll
+    for (int e = 0; e < Row<T>::E; ++e) {
+      const float z = element<T>(from.r[j], e);
+      if (z < bound) continue;
+      const int at = atomicAdd(&sh.found, 1);
+      if (at < CANDIDATES) sh.candidate[at] = rank_key(z, row.index(v, e));
+    }
+  }
+}
+
+// The candidates of a row where the bound let too many through (masked, constant or rising rows): a bound for every tile, and
+// the tile's exact choice where that does not help either.
+template <typename T, int NT> __device__ __noinline__ void careful_candidates(const Row<T> row, int begin, int end, int top, Shared<NT / 32>& sh) {
+  __syncthreads();
+  if (threadIdx.x == 0) sh.found = 0;
+  uint32_t least = 0;
+  int kept = 0;
+  for (int first = begin, parity = 0; first < end; first += U * NT, parity ^= 1) {
+    Tile tile;
+    row.template read<NT>(tile, first, end);
+    const float most = largest_of<T>(tile, (end - first - (int)threadIdx.x + NT - 1) / NT);
+    const uint32_t sorted = part_maxima<NT>(most, top <= FEW, sh.group[parity]);
+    if (NT == 32) __syncthreads();
+    least = max(least, __shfl_sync(ALL, sorted, top - 1));
+    const float bound = value_of(least);
+    if (!(most < bound)) push<T, NT>(row, tile, first, end, bound, sh);
+    __syncthreads();
+    if (sh.found > CANDIDATES) {
+      // no room: the `top` best that earlier tiles left, and this tile's
+      __syncthreads();
+      rank_keys<NT>(sh.candidate, kept, top, [&](uint64_t key, int larger) { sh.best[larger] = key; });
+      __syncthreads();
+      kept = min(kept, top);
+      if ((int)threadIdx.x < kept) sh.candidate[threadIdx.x] = sh.best[threadIdx.x];
+      exact_candidates<T, NT>(row, tile, first, end, top, kept, sh);
+    }
+    kept = sh.found;
+    __syncthreads();
+  }
+}
+
+// One pass over the row, the next vectors on their way while these are added.  Alternatives: a thread whose N vectors reach the
+// bound so far notes where they are; when the bound is final the few that still reach it are looked at again.
 template <typename T, int NT, bool TOP>
 __global__ void __launch_bounds__(NT, 1024 / NT) scores_kernel(const __grid_constant__ ScoreParams p) {
   constexpr int E = Row<T>::E, WARPS = NT / 32;
-  __shared__ Shared<WARPS> sh;
+  __shared__ Sums<WARPS> sums;
+  __shared__ typename std::conditional<TOP, Shared<WARPS>, int>::type sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int share = blockIdx.x % p.split;
   const int64_t n = blockIdx.x / p.split;
   const Row<T> row(p.logits, n, p.row_stride, p.V);
   const int each = (row.vectors + p.split - 1) / p.split, begin = share * each, end = min(begin + each, row.vectors);
-  Stats a{-INFINITY, 0.0f, 0.0f};
-  int kept = 0;                                      // candidates of the tiles so far
+  int kept = 0;                                      // candidates
   if (p.split > 1) cooperative_groups::this_cluster().barrier_arrive();
 
-  if constexpr (!TOP) {
-    // the next vectors are on their way while these are added
-    constexpr int N = U / 2;
-    Vectors<N> now, next;
-    row.template read<NT>(now, begin, end);
-    for (int first = begin; first < end; first += N * NT) {
-      row.template read<NT>(next, first + N * NT, end);
-      const int count = (end - first - (int)threadIdx.x + NT - 1) / NT;
-      float most = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (j < count) most = max_nan(most, largest<T>(now.r[j]));
-      add<T, N>(a, now, count, (end - first + NT - 1) / NT, most);
-      now = next;
-    }
-  } else {
-    if (threadIdx.x == 0) sh.found = 0;
-    uint32_t least = 0;                              // order that at least `top` elements of the row so far reach
-    int parity = 0;
-    for (int first = begin; first < end; first += U * NT, parity ^= 1) {
-      Tile tile;
-      uint4 (&r)[U] = tile.r;
-      row.template read<NT>(tile, first, end);
-      const int count = (end - first - (int)threadIdx.x + NT - 1) / NT;
-      float half[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-      for (int j = 0; j < U; ++j)
-        if (j < count) half[j * 2 / U] = max_nan(half[j * 2 / U], largest<T>(r[j]));
-      const float most = max_nan(half[0], half[1]);
+  Stats a{-INFINITY, 0.0f, 0.0f};
+  const bool has_edge = share == 0 && (int)threadIdx.x < row.edges();
+  const float edge = has_edge ? to_float(row.z[row.edge(threadIdx.x)]) : -INFINITY;
+  if (edge != -INFINITY) {
+    const float y = at_least(exponent(edge, edge)), x = exp2_of(y);
+    a = Stats{edge, x, x * y};
+  }
+  // `top` parts of the tiles seen reach the top-th largest of the parts' maxima: so many elements do, and of any order of the
+  // elements not many more are to be expected (of one tile 32 ln(32 / (32 - top))).  The bound is taken again when as many
+  // tiles have passed as before: it lets about as many through from one time to the next.
+  uint32_t parts = 0;                                // the largest maxima, one a lane
+  float bound = -INFINITY;
+  if constexpr (TOP) {
+    if (threadIdx.x == 0) sh.records = sh.found = 0;
+    if (NT == 32) __syncthreads();
+  }
 
-      // `top` of the 32 parts of the tile reach their top-th largest maximum: so many elements do, and of any order of the
-      // elements not many more are to be expected, 32 ln(32 / (32 - top)).  For more than FEW alternatives 64 parts.
-      const bool few = p.top <= FEW;
-      uint32_t g[2] = {order_of(few ? most : half[0]), order_of(half[1])};
-#pragma unroll
-      for (int o = 1; o < WARPS; o *= 2) g[0] = max(g[0], __shfl_xor_sync(ALL, g[0], o));
-      if (!few) {
-#pragma unroll
-        for (int o = 1; o < WARPS; o *= 2) g[1] = max(g[1], __shfl_xor_sync(ALL, g[1], o));
+  Vectors<N> now, next;
+  row.template read<NT>(now, begin, end);
+  for (int first = begin, i = 0; first < end; first += N * NT, ++i) {
+    row.template read<NT>(next, first + N * NT, end);
+    const int count = (end - first - (int)threadIdx.x + NT - 1) / NT;
+    const float most = largest_of<T>(now, count);
+    add<T, N>(a, now, count, (end - first + NT - 1) / NT, most);
+    if constexpr (TOP) {
+      if ((i & (i + 1)) == 0) {
+        const uint32_t sorted = part_maxima<NT>(most, p.top <= FEW, sh.group[__popc(i) & 1]);
+        parts = i == 0 ? sorted : merge_sorted(parts, sorted);
+        bound = value_of(__shfl_sync(ALL, parts, p.top - 1));
       }
-      if (lane % WARPS == 0) {
-        sh.group[parity][threadIdx.x / WARPS] = g[0];
-        if (!few) sh.group[parity][32 + threadIdx.x / WARPS] = g[1];
-      }
-      add<T, U>(a, tile, count, (end - first + NT - 1) / NT, most);
-      __syncthreads();
-      uint32_t sorted = sort_warp(sh.group[parity][lane]);
-      if (!few) sorted = merge_sorted(sorted, sort_warp(sh.group[parity][32 + lane]));
-      least = max(least, __shfl_sync(ALL, sorted, p.top - 1));
-      const float bound = value_of(least);
       if (!(most < bound)) {
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-          if (largest<T>(r[j]) < bound) continue;
-          const int v = first + j * NT + threadIdx.x;
-          unsigned reach = 0;
-#pragma unroll
-          for (int e = 0; e < E; ++e) reach |= !(element<T>(r[j], e) < bound) && v < end && row.real(row.index(v, e)) ? 1u << e : 0u;
-          for (; reach; reach &= reach - 1) {
-            const int e = __ffs(reach) - 1, at = atomicAdd(&sh.found, 1);
-            const uint32_t w = word(r[j], sizeof(T) == 2 ? e / 2 : e);
-            const float z = __uint_as_float(sizeof(T) == 2 ? (e & 1 ? w & 0xffff0000u : w << 16) : w);
-            if (at < CANDIDATES) sh.candidate[at] = rank_key(z, row.index(v, e));
-          }
+        if (end - begin <= N * NT) {                 // (all there is: nothing to wait for)
+          push<T, NT>(row, now, first, end, bound, sh);
+        } else {
+          const int at = atomicAdd(&sh.records, 1);
+          if (at < RECORDS) sh.record[at] = make_uint2(order_of(most), (uint32_t)(first + threadIdx.x));
         }
       }
-      __syncthreads();
-      if (sh.found > CANDIDATES) {
-        // no room: the `top` best that earlier tiles left, and this tile's
-        __syncthreads();
-        rank_keys<NT>(sh.candidate, kept, p.top, [&](uint64_t key, int larger) { sh.best[larger] = key; });
-        __syncthreads();
-        kept = min(kept, p.top);
-        if ((int)threadIdx.x < kept) sh.candidate[threadIdx.x] = sh.best[threadIdx.x];
-        exact_candidates<T, NT>(row, tile, first, end, p.top, kept, sh);
+    }
+    now = next;
+  }
+
+  if constexpr (TOP) {
+    __syncthreads();
+    const int records = sh.records;
+    if (records <= RECORDS) {
+      const uint32_t least = bound == -INFINITY ? 0 : order_of(bound);
+      for (int q = warp; q < records; q += WARPS) {
+        const uint2 at = sh.record[q];
+        const int v = (int)at.y + lane / E * NT;
+        if (at.x < least || lane >= N * E || v >= end) continue;
+        const float z = to_float(row.z[row.index(v, lane % E)]);
+        if (z < bound) continue;
+        const int to = atomicAdd(&sh.found, 1);
+        if (to < CANDIDATES) sh.candidate[to] = rank_key(z, row.index(v, lane % E));
       }
-      kept = sh.found;
     }
     __syncthreads();
+    if (records > RECORDS || sh.found > CANDIDATES) careful_candidates<T, NT>(row, begin, end, p.top, sh);
+    if (has_edge && !(edge < bound)) sh.candidate[atomicAdd(&sh.found, 1)] = rank_key(edge, row.edge(threadIdx.x));
+    __syncthreads();
+    kept = sh.found;
   }
 
   join<32>(a);
   if constexpr (WARPS > 1) {
-    if (lane == 0) sh.parts[warp] = a;
+    if (lane == 0) sums.parts[warp] = a;
     __syncthreads();
-    a = sh.parts[lane % WARPS];
+    // (the row's results are left to the threads that have a candidate to rank)
+    if (p.split == 1 && warp > 0 && (!TOP || warp * 32 >= kept)) return;
+    a = sums.parts[lane % WARPS];
     join<WARPS>(a);
   }
   if (p.split > 1) {
     // the shares of a row meet in the first CTA of the cluster
     cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
     cluster.barrier_wait();                          // (the first CTA has started)
-    Shared<WARPS>* to = cluster.map_shared_rank(&sh, 0);
-    if (threadIdx.x == 0) to->shares[share] = a;
+    if (threadIdx.x == 0) cluster.map_shared_rank(&sums, 0)->shares[share] = a;
     if constexpr (TOP) {
+      auto* to = cluster.map_shared_rank(&sh, 0);
       if ((int)threadIdx.x >= kept && (int)threadIdx.x < p.top) to->best[share * p.top + threadIdx.x] = 0;      // (fewer found)
       rank_keys<NT>(sh.candidate, kept, p.top, [&](uint64_t key, int larger) { to->best[share * p.top + larger] = key; });
     }
     cluster.sync();
     if (share > 0) return;
-    a = lane < p.split ? sh.shares[lane] : Stats{-INFINITY, 0.0f, 0.0f};
+    a = lane < p.split ? sums.shares[lane] : Stats{-INFINITY, 0.0f, 0.0f};
     join<32>(a);
   }
   const bool empty = a.m == -INFINITY;
@@ -499,12 +556,13 @@ template <typename T, int NT> cudaError_t scores(const ScoreParams& p, cudaStrea
 }
 
 template <typename T> cudaError_t scores(ScoreParams p, cudaStream_t stream) {
-  // Threads for a row: as few as hold it in one tile, so that short rows leave no thread without work; 256 at most.
-  const int64_t vectors = ((int64_t)p.V + 16 / sizeof(T) - 1) / (16 / sizeof(T)) + 1;
+  const int64_t vectors = p.V / (16 / sizeof(T));
   p.split = 1;
-  if (vectors <= 32 * U) return scores<T, 32>(p, stream);
-  if (vectors <= 64 * U) return scores<T, 64>(p, stream);
-  if (vectors <= 128 * U) return scores<T, 128>(p, stream);
+  // Few threads a row where rows are many: what a row costs beside its elements (joins, ranks, barriers) grows with them.  16384
+  // x 32000 bf16, sums: 64 threads 184 us, 128 188, 256 205; with 8 alternatives 281, 275, 320, with 32 498, 393, 430.
+  if (vectors <= 32 * N && p.top <= FEW) return scores<T, 32>(p, stream);
+  if (vectors <= 64 * N || (p.rows >= 2048 && !p.top)) return scores<T, 64>(p, stream);
+  if (vectors <= 128 * N || p.rows >= 1024) return scores<T, 128>(p, stream);
   // Few rows: a row over a cluster of CTAs, a vector a thread at least, up to four CTAs an SM.
   while (p.split < MAX_SPLIT && p.rows * p.split * 2 <= 592 && vectors >= 256 * 2 * p.split) p.split *= 2;
   return scores<T, 256>(p, stream);
@@ -549,12 +607,18 @@ __global__ void __launch_bounds__(NT) scores_grad_kernel(const __grid_constant__
     const Pair e = sizeof(T) == 2 ? pair(exp2_of(y.x), exp2_of(y.y)) : pair(expf(at_least(raw.x)), expf(at_least(raw.y)));
     return both(e * fma(gh2, lp, offset2));
   };
+  if (blockIdx.y == 0 && (int)threadIdx.x < row.edges()) {
+    const int i = row.edge(threadIdx.x);
+    const float z = to_float(row.z[i]);
+    d[i] = from_float<T>(empty ? 0.0f : gradient(pair(z, z)).x);
+  }
   const bool together = (uintptr_t)d % 16 == (uintptr_t)row.z % 16;       // vectors of z are vectors of d
+  const uint4* base = row.base();
   for (int v0 = begin + threadIdx.x; v0 < end; v0 += NT * AHEAD) {
     uint4 r[AHEAD];
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j)
-      if (v0 + j * NT < end) r[j] = row.read(v0 + j * NT);
+      if (v0 + j * NT < end) r[j] = base[v0 + j * NT];
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
       const int v = v0 + j * NT;
@@ -566,13 +630,13 @@ __global__ void __launch_bounds__(NT) scores_grad_kernel(const __grid_constant__
         f[2 * i] = empty ? 0.0f : x.x;
         f[2 * i + 1] = empty ? 0.0f : x.y;
       }
-      if (together && row.whole(v)) {
-        if constexpr (E == 8) store8(d + row.index(v, 0), f);
-        else *reinterpret_cast<float4*>(d + row.index(v, 0)) = make_float4(f[0], f[1], f[2], f[3]);
+      T* to = d + row.index(v, 0);
+      if (together) {
+        if constexpr (E == 8) store8(to, f);
+        else *reinterpret_cast<float4*>(to) = make_float4(f[0], f[1], f[2], f[3]);
       } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (row.real(row.index(v, e))) d[row.index(v, e)] = from_float<T>(f[e]);
+        for (int e = 0; e < E; ++e) to[e] = from_float<T>(f[e]);
       }
     }
   }
@@ -583,8 +647,9 @@ __global__ void __launch_bounds__(NT) scores_grad_kernel(const __grid_constant__
   for (int w = threadIdx.x; w < named; w += NT) {
     const int64_t mine = token(w);
     if (mine < 0 || mine >= p.V) continue;
-    const int v = (int)(mine + row.skew) / E;
-    if (v < begin || v >= end) continue;
+    // (who wrote it first writes it again: the CTA of its vector, or the first one)
+    const int v = mine < row.head ? row.vectors : (int)(mine - row.head) / E;
+    if (v < row.vectors ? v < begin || v >= end : blockIdx.y > 0) continue;
     float own = 0.0f;
     bool first = true;
     for (int k = 0; k < named; ++k) {
