@@ -268,7 +268,9 @@ def lib() -> ctypes.CDLL:
 # entry points of the C ABI that the host-side extension calls, in the order of its table
 _NATIVE_ENTRIES = ("fpb_retention_fwd", "fpb_retention_bwd", "fpb_pop_retention_fwd", "fpb_pop_retention_bwd", "fpb_pop_suffix_fwd",
                    "fpb_pop_suffix_bwd", "fpb_retention_step", "fpb_workspace_bytes", "fpb_rotary", "fpb_groupnorm_gate_fwd",
-                   "fpb_groupnorm_gate_bwd", "fpb_layernorm_fwd", "fpb_layernorm_bwd", "fpb_column_sums")
+                   "fpb_groupnorm_gate_bwd", "fpb_layernorm_fwd", "fpb_layernorm_bwd", "fpb_column_sums", "fpb_qk_norm_rotary_fwd",
+                   "fpb_qk_norm_rotary_bwd", "fpb_dropout", "fpb_embedding_fwd", "fpb_embedding_workspace", "fpb_embedding_bwd",
+                   "fpb_token_scores_fwd", "fpb_token_scores_bwd")
 _native = None
 _native_bound: Optional[ctypes.CDLL] = None
 _WITHOUT_NATIVE = "the operators' calls go through Python, 50 to 65 us each"

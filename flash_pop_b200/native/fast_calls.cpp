@@ -38,6 +38,14 @@ struct Entry {
   decltype(&fpb_layernorm_fwd) norm_fwd;
   decltype(&fpb_layernorm_bwd) norm_bwd;
   decltype(&fpb_column_sums) column_sums;
+  decltype(&fpb_qk_norm_rotary_fwd) qk_norm_fwd;
+  decltype(&fpb_qk_norm_rotary_bwd) qk_norm_bwd;
+  decltype(&fpb_dropout) dropout;
+  decltype(&fpb_embedding_fwd) embedding_fwd;
+  decltype(&fpb_embedding_workspace) embedding_workspace;
+  decltype(&fpb_embedding_bwd) embedding_bwd;
+  decltype(&fpb_token_scores_fwd) scores_fwd;
+  decltype(&fpb_token_scores_bwd) scores_bwd;
 } entry;
 constexpr int ENTRIES = sizeof(Entry) / sizeof(void*), MAX_HEADS = 256;
 
@@ -482,6 +490,181 @@ PyObject* column_sums(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+double real_number(PyObject* o) {
+  NEED(PyFloat_Check(o));
+  return PyFloat_AS_DOUBLE(o);
+}
+PyObject* status_or(int r, std::initializer_list<at::Tensor> ts) { return r ? PyLong_FromLong(r) : tuple_of(ts); }
+
+// queries and keys (B, T, heads, d) with the weights (d, fp32) and phasors of their norm and rotation
+struct QkNorm {
+  at::Tensor q, k, wq, wk, ph;
+  int32_t B, T, Hq, Hk, d;
+  int64_t step;
+  QkNorm(PyObject* const* a) : q(tensor(a[0])), k(tensor(a[1])), wq(maybe(a[2])), wk(maybe(a[3])), ph(maybe(a[4])) {
+    NEED(q.dim() == 4 && k.dim() == 4 && q.size(0) == k.size(0) && q.size(1) == k.size(1) && q.size(3) == k.size(3) && q.size(3) % 8 == 0 && q.size(3) <= 256);
+    NEED(q.numel() < INT32_MAX && k.numel() < INT32_MAX);
+    B = (int32_t)q.size(0); T = (int32_t)q.size(1); Hq = (int32_t)q.size(2); Hk = (int32_t)k.size(2); d = (int32_t)q.size(3);
+    NEED(real(q.scalar_type()) && k.scalar_type() == q.scalar_type() && k.device() == q.device());
+    step = 0;
+    if (ph.defined()) {
+      NEED(ph.dim() == 4 && (ph.size(0) == 1 || ph.size(0) == B) && ph.size(1) == T && ph.size(2) == d / 2 && ph.size(3) == 2 && ph.is_contiguous() &&
+           ph.scalar_type() == at::kFloat && ph.device() == q.device() && (uintptr_t)ph.data_ptr() % 16 == 0);
+      step = ph.size(0) == 1 ? 0 : (int64_t)T * (d / 2);
+    }
+    ready(q); ready(k);
+  }
+  void ready(const at::Tensor& t) const { NEED(t.scalar_type() == q.scalar_type() && t.device() == q.device() && in_place(t) && aligned(t, 16)); }
+  const float* weight(const at::Tensor& w) const { return param(w, d, q); }
+  const float* phasors() const { return ph.defined() ? (const float*)ph.data_ptr() : nullptr; }
+};
+// qk_norm_forward(q, k, wq, wk, phasors, eps) -> (yq, yk)
+PyObject* qk_norm_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 6, [&]() -> PyObject* {
+    const QkNorm c(a);
+    const float eps = (float)real_number(a[5]), *wq = c.weight(c.wq), *wk = c.weight(c.wk);
+    Place here(c.q);
+    const at::Tensor yq = make(c.q.sizes(), c.q, c.q.scalar_type()), yk = make(c.k.sizes(), c.q, c.q.scalar_type());
+    const fpb_seq sq = seq(c.q), sk = seq(c.k), oq = seq(yq), ok = seq(yk);
+    const int r = unlocked([&] {
+      return entry.qk_norm_fwd(c.B, c.T, c.Hq, c.Hk, c.d, code(c.q.scalar_type()), eps, wq, wk, c.phasors(), c.step, &sq, &sk, &oq, &ok, here.stream);
+    });
+    return status_or(r, {yq, yk});
+  });
+}
+// qk_norm_backward(q, k, wq, wk, phasors, eps, dyq, dyk, need_wq, need_wk) -> (dq, dk, dwq, dwk)
+PyObject* qk_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 10, [&]() -> PyObject* {
+    const QkNorm c(a);
+    const float eps = (float)real_number(a[5]), *wq = c.weight(c.wq), *wk = c.weight(c.wk);
+    const at::Tensor dyq = tensor(a[6]), dyk = tensor(a[7]);
+    NEED(dyq.sizes() == c.q.sizes() && dyk.sizes() == c.k.sizes());
+    c.ready(dyq); c.ready(dyk);
+    Place here(c.q);
+    const at::Tensor dq = make(c.q.sizes(), c.q, c.q.scalar_type()), dk = make(c.k.sizes(), c.q, c.q.scalar_type()),
+                     dwq = a[8] == Py_True ? make({c.d}, c.q, at::kFloat) : at::Tensor(), dwk = a[9] == Py_True ? make({c.d}, c.q, at::kFloat) : at::Tensor(),
+                     scratch = make({FPB_QK_NORM_SCRATCH(c.d)}, c.q, at::kByte);
+    const fpb_seq sq = seq(c.q), sk = seq(c.k), gq = seq(dyq), gk = seq(dyk), oq = seq(dq), ok = seq(dk);
+    const int r = unlocked([&] {
+      return entry.qk_norm_bwd(c.B, c.T, c.Hq, c.Hk, c.d, code(c.q.scalar_type()), eps, wq, wk, c.phasors(), c.step, &sq, &sk, &gq, &gk, &oq, &ok,
+                               dwq.defined() ? (float*)dwq.data_ptr() : nullptr, dwk.defined() ? (float*)dwk.data_ptr() : nullptr, scratch.data_ptr(),
+                               here.stream);
+    });
+    return status_or(r, {dq, dk, dwq, dwk});
+  });
+}
+
+// dropout(x, residual or None, p, seed) -> (y,)
+PyObject* dropout(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 4, [&]() -> PyObject* {
+    const at::Tensor x = tensor(a[0]), res = maybe(a[1]), seed = tensor(a[3]);
+    const double p = real_number(a[2]);
+    NEED(real(x.scalar_type()) && x.is_contiguous() && p >= 0.0 && p <= 1.0);
+    if (res.defined()) NEED(res.scalar_type() == x.scalar_type() && res.sizes() == x.sizes() && res.is_contiguous() && res.device() == x.device());
+    NEED(seed.scalar_type() == at::kLong && seed.numel() == 1 && seed.device() == x.device());
+    Place here(x);
+    const at::Tensor y = make(x.sizes(), x, x.scalar_type());
+    const int r = unlocked([&] {
+      return entry.dropout(x.numel(), code(x.scalar_type()), p, (const int64_t*)seed.data_ptr(), x.data_ptr(), res.defined() ? res.data_ptr() : nullptr,
+                           y.data_ptr(), here.stream);
+    });
+    return status_or(r, {y});
+  });
+}
+
+int64_t pitch(const at::Tensor& t) {             // of a matrix whose rows can be read in place
+  NEED(t.dim() == 2 && (t.stride(1) == 1 || t.size(1) == 1) && (t.size(0) == 1 || t.stride(0) >= t.size(1)));
+  return t.size(0) > 1 ? t.stride(0) : t.size(1);
+}
+at::Tensor ids(PyObject* o, const at::Tensor& like) {
+  const at::Tensor t = tensor(o);
+  NEED(t.scalar_type() == at::kLong && t.is_contiguous() && t.device() == like.device());
+  return t;
+}
+// embedding_forward(tokens, weight, scale) -> (y,)
+PyObject* embedding_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 3, [&]() -> PyObject* {
+    const at::Tensor w = tensor(a[1]), t = ids(a[0], w);
+    const float scale = (float)real_number(a[2]);
+    NEED(real(w.scalar_type()));
+    const int64_t stride = pitch(w), D = w.size(1);
+    NEED(D <= 1 << 20);
+    std::vector<int64_t> shape(t.sizes().begin(), t.sizes().end());
+    shape.push_back(D);
+    Place here(w);
+    const at::Tensor y = make(shape, w, w.scalar_type());
+    const int r = unlocked([&] {
+      return entry.embedding_fwd(t.numel(), w.size(0), (int32_t)D, code(w.scalar_type()), (const int64_t*)t.data_ptr(), w.data_ptr(), stride, scale,
+                                 y.data_ptr(), here.stream);
+    });
+    return status_or(r, {y});
+  });
+}
+// embedding_backward(tokens, dy (..., D), V, padding, scale) -> (dw,)
+PyObject* embedding_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 5, [&]() -> PyObject* {
+    const at::Tensor dy = tensor(a[1]), t = ids(a[0], dy);
+    const int64_t V = integer(a[2]), padding = integer(a[3]), N = t.numel(), D = dy.size(-1);
+    const float scale = (float)real_number(a[4]);
+    NEED(real(dy.scalar_type()) && dy.is_contiguous() && dy.numel() == N * D && V > 0 && D <= 1 << 20);
+    Place here(dy);
+    const at::Tensor dw = make({V, D}, dy, dy.scalar_type());
+    const int64_t need = entry.embedding_workspace(N, V, (int32_t)D);
+    const at::Tensor scratch = make({need}, dy, at::kByte);
+    const int r = unlocked([&] {
+      return entry.embedding_bwd(N, V, (int32_t)D, code(dy.scalar_type()), (const int64_t*)t.data_ptr(), padding, scale, dy.data_ptr(), D, dw.data_ptr(),
+                                 scratch.data_ptr(), need, here.stream);
+    });
+    return status_or(r, {dw});
+  });
+}
+
+// scores_forward(logits (..., V), tokens (...), top) -> (logprob, entropy, stats, top_logprob or None, top_tokens or None)
+PyObject* scores_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 3, [&]() -> PyObject* {
+    const at::Tensor z = tensor(a[0]), t = ids(a[1], z);
+    const int64_t top = integer(a[2]);
+    NEED(z.dim() >= 1 && t.sizes() == z.sizes().slice(0, z.dim() - 1) && real(z.scalar_type()) && (z.is_contiguous() || z.dim() == 2));
+    const int64_t V = z.size(-1), rows = t.numel(), stride = z.is_contiguous() ? V : pitch(z);
+    NEED(top >= 0 && top <= FPB_MAX_TOP && top <= V && V <= 1 << 30);
+    Place here(z);
+    const at::Tensor lp = make(t.sizes(), z, at::kFloat), h = make(t.sizes(), z, at::kFloat), stats = make({rows, 2}, z, at::kFloat);
+    at::Tensor tl, tt;
+    if (top) {
+      std::vector<int64_t> shape(t.sizes().begin(), t.sizes().end());
+      shape.push_back(top);
+      tl = make(shape, z, at::kFloat);
+      tt = make(shape, z, at::kLong);
+    }
+    const int r = unlocked([&] {
+      return entry.scores_fwd(rows, (int32_t)V, code(z.scalar_type()), (int32_t)top, z.data_ptr(), stride, (const int64_t*)t.data_ptr(), (float*)lp.data_ptr(),
+                              (float*)h.data_ptr(), (float*)stats.data_ptr(), top ? (float*)tl.data_ptr() : nullptr,
+                              top ? (int64_t*)tt.data_ptr() : nullptr, here.stream);
+    });
+    return status_or(r, {lp, h, stats, tl, tt});
+  });
+}
+// scores_backward(logits, tokens, entropy, stats, top_tokens or None, g_logprob, g_entropy, g_top (each or None)) -> (d,)
+PyObject* scores_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 8, [&]() -> PyObject* {
+    const at::Tensor z = tensor(a[0]), t = ids(a[1], z), h = tensor(a[2]), stats = tensor(a[3]), tt = maybe(a[4]);
+    const at::Tensor g[3] = {maybe(a[5]), maybe(a[6]), maybe(a[7])};
+    NEED(z.is_contiguous() || z.dim() == 2);
+    const int64_t V = z.size(-1), rows = t.numel(), stride = z.is_contiguous() ? V : pitch(z), top = tt.defined() ? tt.size(-1) : 0;
+    for (int i = 0; i < 3; ++i)
+      if (g[i].defined())
+        NEED(g[i].scalar_type() == at::kFloat && g[i].is_contiguous() && g[i].device() == z.device() && g[i].numel() == (i < 2 ? rows : rows * top));
+    Place here(z);
+    const at::Tensor d = make(z.sizes(), z, z.scalar_type());
+    auto at = [](const at::Tensor& x) { return x.defined() ? (const float*)x.data_ptr() : nullptr; };
+    const int r = unlocked([&] {
+      return entry.scores_bwd(rows, (int32_t)V, code(z.scalar_type()), (int32_t)top, z.data_ptr(), stride, (const int64_t*)t.data_ptr(), at(h), at(stats),
+                              tt.defined() ? (const int64_t*)tt.data_ptr() : nullptr, at(g[0]), at(g[1]), at(g[2]), d.data_ptr(), V, here.stream);
+    });
+    return status_or(r, {d});
+  });
+}
+
 // address(t, dtype, align, device_index, n0, n1) -> address of a contiguous parameter of that shape (n1 = 0: one dimension), or None
 PyObject* address(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded(n, 6, [&]() -> PyObject* {
@@ -522,7 +705,8 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(step), FAST(forward), FAST(backward), FAST(suffix_forward), FAST(suffix_backward), FAST(rotary), FAST(gate_forward),
-                         FAST(gate_backward), FAST(norm_forward), FAST(norm_backward), FAST(column_sums), FAST(address), FAST(wanted), FAST(bind), {nullptr, nullptr, 0, nullptr}};
+                         FAST(gate_backward), FAST(norm_forward), FAST(norm_backward), FAST(column_sums), FAST(qk_norm_forward), FAST(qk_norm_backward),
+                         FAST(dropout), FAST(embedding_forward), FAST(embedding_backward), FAST(scores_forward), FAST(scores_backward), FAST(address), FAST(wanted), FAST(bind), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "fpb_fast_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

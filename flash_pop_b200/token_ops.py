@@ -10,15 +10,14 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from flash_pop_b200 import _lib
-from flash_pop_b200.layer_ops import _OK_DTYPES, _ptr
+from flash_pop_b200.layer_ops import _OK_DTYPES, _ptr, no_graph
 
 MAX_TOP = 32
 
 
-def _ids(tokens: Tensor, like: Tensor, name: str) -> Tensor:
+def _check_ids(tokens: Tensor, like: Tensor) -> None:
     if tokens.dtype not in (torch.int64, torch.int32) or tokens.device != like.device:
-        raise ValueError(f"{name}: int64 or int32 ids on {like.device}; got {tokens.dtype} on {tokens.device}")
-    return tokens.to(torch.int64)
+        raise ValueError(f"tokens: int64 or int32 ids on {like.device}; got {tokens.dtype} on {tokens.device}")
 
 
 def _matrix(t: Tensor) -> Tensor:
@@ -34,6 +33,13 @@ def _pitch(t: Tensor) -> int:
 class Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, tokens, weight, scale, padding):
+        fast = _lib.result(_lib.native().embedding_forward(tokens, weight, scale))
+        if fast is not None:
+            ctx.save_for_backward(tokens)
+            ctx.of = *weight.shape, weight.dtype, scale, padding
+            return fast[0]
+        _check_embedding(tokens, weight)
+        tokens = tokens.to(torch.int64)
         w, ids = _matrix(weight), tokens.contiguous()
         V, D = w.shape
         N = ids.numel()
@@ -50,6 +56,10 @@ class Embedding(torch.autograd.Function):
     def backward(ctx, dy):
         (ids,) = ctx.saved_tensors
         V, D, dtype, scale, padding = ctx.of
+        if dy.dtype == dtype:
+            fast = _lib.result(_lib.native().embedding_backward(ids, dy, V, padding, scale))
+            if fast is not None:
+                return None, fast[0], None, None
         N = ids.numel()
         dy = _matrix(dy.to(dtype).reshape(N, D))
         dw = torch.empty((V, D), device=dy.device, dtype=dtype)
@@ -61,19 +71,30 @@ class Embedding(torch.autograd.Function):
         return None, dw, None, None
 
 
-def embedding(tokens: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> Tensor:
-    """``weight[tokens] * scale`` for ids of any shape and a (V, D) table, in the table's dtype.  An id outside [0, V) gives a zero
-    row and has no part in the gradient.  The gradient of the table is dense; rows are summed in fp32 in the order of the
-    ids and rounded once, so it is the same every time.  `padding_idx` (negative: from the end): its row gets no gradient."""
+def _check_embedding(tokens: Tensor, weight: Tensor) -> None:
     _lib.require_cuda(tokens, weight)
     if weight.dim() != 2 or weight.size(0) == 0 or weight.size(1) == 0:
         raise ValueError(f"weight: (V, D), neither 0; got {tuple(weight.shape)}")
     if weight.dtype not in _OK_DTYPES:
         raise ValueError(f"weight: bfloat16 or float32; got {weight.dtype}")
-    V = weight.size(0)
-    if padding_idx is not None and not -V <= padding_idx < V:
-        raise ValueError(f"padding_idx {padding_idx} outside a table of {V} rows")
-    return Embedding.apply(_ids(tokens, weight, "tokens"), weight, float(scale), -1 if padding_idx is None else padding_idx % V)
+    _check_ids(tokens, weight)
+
+
+def embedding(tokens: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> Tensor:
+    """``weight[tokens] * scale`` for ids of any shape and a (V, D) table, in the table's dtype.  An id outside [0, V) gives a zero
+    row and has no part in the gradient.  The gradient of the table is dense; rows are summed in fp32 in the order of the
+    ids and rounded once, so it is the same every time.  `padding_idx` (negative: from the end): its row gets no gradient."""
+    scale, padding = float(scale), -1
+    if padding_idx is not None:
+        V = weight.size(0)
+        if not -V <= padding_idx < V:
+            raise ValueError(f"padding_idx {padding_idx} outside a table of {V} rows")
+        padding = padding_idx % V
+    if no_graph(weight):
+        fast = _lib.result(_lib.native().embedding_forward(tokens, weight, scale))
+        if fast is not None:
+            return fast[0]
+    return Embedding.apply(tokens, weight, scale, padding)
 
 
 class TokenScores(NamedTuple):
@@ -83,18 +104,38 @@ class TokenScores(NamedTuple):
     top_tokens: Optional[Tensor]          # (..., top) int64
 
 
+def _check_scores(logits: Tensor, tokens: Tensor, top: int) -> None:
+    _lib.require_cuda(logits, tokens)
+    if logits.dim() < 1 or tokens.shape != logits.shape[:-1]:
+        raise ValueError(f"logits (..., V) and tokens (...): got {tuple(logits.shape)} and {tuple(tokens.shape)}")
+    V = logits.size(-1)
+    if V == 0:
+        raise ValueError("logits over no tokens")
+    if logits.dtype not in _OK_DTYPES:
+        raise ValueError(f"logits: bfloat16 or float32; got {logits.dtype}")
+    if not 0 <= top <= min(MAX_TOP, V):
+        raise ValueError(f"top: 0 to {min(MAX_TOP, V)} of {V} tokens; got {top}")
+    _check_ids(tokens, logits)
+
+
 class _TokenScores(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top):
-        rows, V = logits.shape
-        dev = logits.device
-        new = lambda *shape, dtype=torch.float32: torch.empty(shape, device=dev, dtype=dtype)
-        logprob, entropy, stats = new(rows), new(rows), new(rows, 2)
-        top_logprob, top_tokens = (new(rows, top), new(rows, top, dtype=torch.int64)) if top else (None, None)
-        with torch.cuda.device(dev):
-            _lib.check(_lib.lib().fpb_token_scores_fwd(rows, V, _lib.dtype_code(logits), top, _ptr(logits), _pitch(logits), _ptr(tokens),
-                                                       _ptr(logprob), _ptr(entropy), _ptr(stats), _ptr(top_logprob), _ptr(top_tokens),
-                                                       _lib.stream_ptr(dev)))
+        fast = _lib.result(_lib.native().scores_forward(logits, tokens, top))
+        if fast is not None:
+            logprob, entropy, stats, top_logprob, top_tokens = fast
+        else:
+            _check_scores(logits, tokens, top)
+            shape, V = tokens.shape, logits.size(-1)
+            tokens, z = tokens.to(torch.int64).reshape(-1).contiguous(), _matrix(logits.reshape(-1, V))
+            rows, dev = tokens.numel(), z.device
+            new = lambda *extra, dtype=torch.float32: torch.empty((*shape, *extra), device=dev, dtype=dtype)
+            logprob, entropy, stats = new(), new(), torch.empty((rows, 2), device=dev, dtype=torch.float32)
+            top_logprob, top_tokens = (new(top), new(top, dtype=torch.int64)) if top else (None, None)
+            with torch.cuda.device(dev):
+                _lib.check(_lib.lib().fpb_token_scores_fwd(rows, V, _lib.dtype_code(z), top, _ptr(z), _pitch(z), _ptr(tokens), _ptr(logprob),
+                                                           _ptr(entropy), _ptr(stats), _ptr(top_logprob), _ptr(top_tokens), _lib.stream_ptr(dev)))
+            logits = z.view(logits.shape) if z.is_contiguous() else logits
         ctx.save_for_backward(logits, tokens, entropy, stats, top_tokens)
         ctx.set_materialize_grads(False)
         if top:
@@ -107,14 +148,18 @@ class _TokenScores(torch.autograd.Function):
         logits, tokens, entropy, stats, top_tokens = ctx.saved_tensors
         if g_logprob is None and g_entropy is None and g_top is None:
             return None, None, None
-        rows, V = logits.shape
+        fast = _lib.result(_lib.native().scores_backward(logits, tokens, entropy, stats, top_tokens, g_logprob, g_entropy, g_top))
+        if fast is not None:
+            return fast[0], None, None
+        V = logits.size(-1)
+        z = _matrix(logits.reshape(-1, V))
+        rows = z.size(0)
         g_logprob, g_entropy, g_top = (None if g is None else g.to(torch.float32).contiguous() for g in (g_logprob, g_entropy, g_top))
-        d = torch.empty((rows, V), device=logits.device, dtype=logits.dtype)
-        with torch.cuda.device(logits.device):
-            _lib.check(_lib.lib().fpb_token_scores_bwd(rows, V, _lib.dtype_code(logits), 0 if top_tokens is None else top_tokens.size(1),
-                                                       _ptr(logits), _pitch(logits), _ptr(tokens), _ptr(entropy), _ptr(stats),
-                                                       _ptr(top_tokens), _ptr(g_logprob), _ptr(g_entropy), _ptr(g_top), _ptr(d), V,
-                                                       _lib.stream_ptr(logits.device)))
+        d = torch.empty(logits.shape, device=z.device, dtype=z.dtype)
+        with torch.cuda.device(z.device):
+            _lib.check(_lib.lib().fpb_token_scores_bwd(rows, V, _lib.dtype_code(z), 0 if top_tokens is None else top_tokens.size(-1), _ptr(z), _pitch(z),
+                                                       _ptr(tokens), _ptr(entropy), _ptr(stats), _ptr(top_tokens), _ptr(g_logprob), _ptr(g_entropy),
+                                                       _ptr(g_top), _ptr(d), V, _lib.stream_ptr(z.device)))
         return d, None, None
 
 
@@ -123,16 +168,8 @@ def token_scores(logits: Tensor, tokens: Tensor, top: int = 0) -> TokenScores:
     tokens with their log probabilities, equal logits by index; fp32 arithmetic, one read of the logits.  All but the indices are
     differentiable (one more read and one write).  A token outside [0, V) has the log probability 0 and sends no gradient
     (`cross_entropy`'s rule).  A row of -inf only gives -inf, entropy 0 and no gradient; NaN or +inf in a row make its numbers NaN."""
-    _lib.require_cuda(logits, tokens)
-    if logits.dim() < 1 or tokens.shape != logits.shape[:-1]:
-        raise ValueError(f"logits (..., V) and tokens (...): got {tuple(logits.shape)} and {tuple(tokens.shape)}")
-    V = logits.size(-1)
-    if logits.dtype not in _OK_DTYPES:
-        raise ValueError(f"logits: bfloat16 or float32; got {logits.dtype}")
-    if not 0 <= top <= min(MAX_TOP, V):
-        raise ValueError(f"top: 0 to {min(MAX_TOP, V)} of {V} tokens; got {top}")
-    if V == 0:
-        raise ValueError("logits over no tokens")
-    ids = _ids(tokens, logits, "tokens").reshape(-1).contiguous()
-    found = _TokenScores.apply(_matrix(logits.reshape(-1, V)), ids, int(top))
-    return TokenScores(*(None if t is None else t.view((*tokens.shape, *t.shape[1:])) for t in found))
+    if no_graph(logits):
+        fast = _lib.result(_lib.native().scores_forward(logits, tokens, top))
+        if fast is not None:
+            return TokenScores(fast[0], fast[1], fast[3], fast[4])
+    return TokenScores(*_TokenScores.apply(logits, tokens, top))
