@@ -270,7 +270,7 @@ _NATIVE_ENTRIES = ("fpb_retention_fwd", "fpb_retention_bwd", "fpb_pop_retention_
                    "fpb_pop_suffix_bwd", "fpb_retention_step", "fpb_workspace_bytes", "fpb_rotary", "fpb_groupnorm_gate_fwd",
                    "fpb_groupnorm_gate_bwd", "fpb_layernorm_fwd", "fpb_layernorm_bwd", "fpb_column_sums", "fpb_qk_norm_rotary_fwd",
                    "fpb_qk_norm_rotary_bwd", "fpb_dropout", "fpb_embedding_fwd", "fpb_embedding_workspace", "fpb_embedding_bwd",
-                   "fpb_token_scores_fwd", "fpb_token_scores_bwd")
+                   "fpb_token_scores_fwd", "fpb_token_scores_bwd", "fpb_strerror")
 _native = None
 _native_bound: Optional[ctypes.CDLL] = None
 _WITHOUT_NATIVE = "the operators' calls go through Python, 50 to 65 us each"

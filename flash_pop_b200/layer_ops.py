@@ -92,13 +92,6 @@ def _check_qk_norm(q: Tensor, k: Tensor, q_weight: Optional[Tensor], k_weight: O
         raise ValueError("q, k, the weights and the phasors have to be on one device")
 
 
-def no_graph(*tensors) -> bool:
-    """Whether a call on these tensors leaves nothing to differentiate, so that no autograd node is made."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return False
-    return getattr(torch.autograd.forward_ad, "_current_level", 0) < 0
-
-
 def _norm_weight(w: Optional[Tensor]) -> Optional[Tensor]:
     if w is None:
         return None
@@ -109,11 +102,6 @@ def _norm_weight(w: Optional[Tensor]) -> Optional[Tensor]:
 class QKNormRotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, phasors, eps):
-        fast = _lib.result(_lib.native().qk_norm_forward(q, k, q_weight, k_weight, phasors, eps))
-        if fast is not None:
-            ctx.save_for_backward(q, k, q_weight, k_weight, phasors)
-            ctx.eps, ctx.step = eps, 0 if phasors is None or phasors.size(0) == 1 else phasors.size(1) * phasors.size(2)
-            return fast
         _check_qk_norm(q, k, q_weight, k_weight, phasors)
         if phasors is not None:
             phasors = phasors.contiguous()
@@ -136,9 +124,6 @@ class QKNormRotary(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dyq, dyk):
         q, k, q_weight, k_weight, phasors = ctx.saved_tensors
-        fast = _lib.result(_lib.native().qk_norm_backward(q, k, q_weight, k_weight, phasors, ctx.eps, dyq, dyk, *ctx.needs_input_grad[2:4]))
-        if fast is not None:
-            return *fast, None, None
         B, T, Hq, d = q.shape
         Hk = k.size(2)
         dyq, dyk = _aligned(dyq.to(q.dtype), 16), _aligned(dyk.to(q.dtype), 16)
@@ -160,10 +145,9 @@ def qk_norm_rotary(q: Tensor, k: Tensor, q_weight: Optional[Tensor], k_weight: O
     (d elements each, None: ones) are shared by the heads; d a multiple of 8, at most 256.  fp32 arithmetic, results in q's dtype.
     No gradient goes to the phasors; the weights' gradients are summed in a fixed order."""
     eps = float(eps)
-    if no_graph(q, k, q_weight, k_weight):
-        fast = _lib.result(_lib.native().qk_norm_forward(q, k, q_weight, k_weight, phasors, eps))
-        if fast is not None:
-            return fast
+    fast = _lib.result(_lib.native().qk_norm_rotary(q, k, q_weight, k_weight, phasors, eps))
+    if fast is not None:
+        return fast
     for w in (q_weight, k_weight):
         if w is not None and w.dtype != torch.float32:           # (their gradients go back through the casts)
             _check_qk_norm(q, k, q_weight, k_weight, phasors)
@@ -177,9 +161,6 @@ def _flat(t: Tensor) -> Tensor:
 
 
 def _drop(x: Tensor, p: float, seed: Tensor, residual: Optional[Tensor]) -> Tensor:
-    fast = _lib.result(_lib.native().dropout(x, residual, p, seed))
-    if fast is not None:
-        return fast[0]
     x, residual = _flat(x), None if residual is None else _flat(residual)
     y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     with torch.cuda.device(x.device):
@@ -207,10 +188,9 @@ def dropout(x: Tensor, p: float, seed: Tensor, residual: Optional[Tensor] = None
     int64 on x's device, and of the element's place alone: no mask is stored, and a captured graph draws another one when the seed's
     content changes.  p counts in steps of 2^-16; what is dropped is 0 whatever it was.  The seed must keep its content until the
     backward has run."""
-    if no_graph(x, residual):
-        fast = _lib.result(_lib.native().dropout(x, residual, float(p), seed))
-        if fast is not None:
-            return fast[0]
+    fast = _lib.result(_lib.native().dropout(x, residual, float(p), seed))
+    if fast is not None:
+        return fast[0]
     _lib.require_cuda(x, seed, residual)
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"p has to be a probability; got {p}")

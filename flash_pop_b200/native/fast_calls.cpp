@@ -16,6 +16,9 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/DynamicTypes.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -46,6 +49,7 @@ struct Entry {
   decltype(&fpb_embedding_bwd) embedding_bwd;
   decltype(&fpb_token_scores_fwd) scores_fwd;
   decltype(&fpb_token_scores_bwd) scores_bwd;
+  decltype(&fpb_strerror) strerror;
 } entry;
 constexpr int ENTRIES = sizeof(Entry) / sizeof(void*), MAX_HEADS = 256;
 
@@ -190,6 +194,9 @@ template <typename F> PyObject* guarded(Py_ssize_t got, Py_ssize_t want, F body)
   } catch (const c10::OutOfMemoryError& e) {
     // (the Python path raises the allocator's own exception type with its message)
     Py_RETURN_NONE;
+  } catch (python_error& e) {
+    e.restore();                                 // (a saved-tensor hook's own)
+    return nullptr;
   } catch (const std::exception& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
     return nullptr;
@@ -490,85 +497,173 @@ PyObject* column_sums(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---- operators with autograd nodes of their own ---------------------------------------------------------------------
+// A small call's gradient through torch.autograd.Function costs 40 to 60 us of Python, several times its kernels; these nodes are C++.
+// Each forward comes in two parts: `run`, which checks and computes and throws NotOurs for what is left to Python, and a node around
+// it where a gradient is recorded.  A backward takes whatever strides the gradients have, by copying them.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+typedef std::vector<at::Tensor> Tensors;
+
+struct Status { int code; };                     // thrown by `run`: a status of the C ABI
+void ran(int status) { if (status) throw Status{status}; }
+void ran_backward(int status) { TORCH_CHECK(status == 0, "flash_pop_b200: ", entry.strerror(status)); }
+
+bool graph_wanted(std::initializer_list<at::Tensor> ts) {
+  for (const at::Tensor& t : ts)
+    if (t.defined()) NEED(!t._fw_grad(0).defined());             // (forward-mode gradients: Python says that there are none)
+  if (!at::GradMode::is_enabled()) return false;
+  for (const at::Tensor& t : ts)
+    if (t.defined() && t.requires_grad()) return true;
+  return false;
+}
+// body, with a status of the C ABI as an int
+template <typename F> PyObject* guarded_call(Py_ssize_t got, Py_ssize_t want, F body) {
+  return guarded(got, want, [&]() -> PyObject* {
+    try {
+      const Tensors out = body();
+      PyObject* r = PyTuple_New((Py_ssize_t)out.size());
+      for (size_t i = 0; r && i < out.size(); ++i) {
+        PyObject* o = wrap(out[i]);
+        if (!o) { Py_DECREF(r); return nullptr; }
+        PyTuple_SET_ITEM(r, (Py_ssize_t)i, o);
+      }
+      return r;
+    } catch (const Status& s) {
+      return PyLong_FromLong(s.code);
+    }
+  });
+}
+// What a backward returns where a graph of it is recorded: a second derivative raises.
+variable_list once(variable_list out, bool graph) {
+  if (!graph) return out;
+  variable_list in;
+  for (const at::Tensor& t : out) in.push_back(t.defined() ? t.detach().requires_grad_(true) : t);
+  return torch::autograd::DelayedError("trying to differentiate twice a function that was marked with @once_differentiable", (int64_t)in.size())
+      .apply(std::move(in));
+}
+at::Tensor dense(const at::Tensor& t) {          // contiguous and 16-byte aligned
+  const at::Tensor c = t.contiguous();
+  return (uintptr_t)c.data_ptr() % 16 ? c.clone() : c;
+}
+at::Tensor readable(const at::Tensor& t) {       // rows as the kernels take them, copied if need be
+  if (t.numel() == 0 || (in_place(t) && aligned(t, 16))) return t;
+  return dense(t);
+}
+// (an absent tensor is no input of a node, nor counted among them)
+typedef std::optional<at::Tensor> Maybe;
+Maybe given(const at::Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); }
+at::Tensor or_none(const Maybe& t) { return t ? *t : at::Tensor(); }
 double real_number(PyObject* o) {
   NEED(PyFloat_Check(o));
   return PyFloat_AS_DOUBLE(o);
 }
-PyObject* status_or(int r, std::initializer_list<at::Tensor> ts) { return r ? PyLong_FromLong(r) : tuple_of(ts); }
 
 // queries and keys (B, T, heads, d) with the weights (d, fp32) and phasors of their norm and rotation
-struct QkNorm {
-  at::Tensor q, k, wq, wk, ph;
-  int32_t B, T, Hq, Hk, d;
-  int64_t step;
-  QkNorm(PyObject* const* a) : q(tensor(a[0])), k(tensor(a[1])), wq(maybe(a[2])), wk(maybe(a[3])), ph(maybe(a[4])) {
-    NEED(q.dim() == 4 && k.dim() == 4 && q.size(0) == k.size(0) && q.size(1) == k.size(1) && q.size(3) == k.size(3) && q.size(3) % 8 == 0 && q.size(3) <= 256);
-    NEED(q.numel() < INT32_MAX && k.numel() < INT32_MAX);
-    B = (int32_t)q.size(0); T = (int32_t)q.size(1); Hq = (int32_t)q.size(2); Hk = (int32_t)k.size(2); d = (int32_t)q.size(3);
-    NEED(real(q.scalar_type()) && k.scalar_type() == q.scalar_type() && k.device() == q.device());
-    step = 0;
-    if (ph.defined()) {
-      NEED(ph.dim() == 4 && (ph.size(0) == 1 || ph.size(0) == B) && ph.size(1) == T && ph.size(2) == d / 2 && ph.size(3) == 2 && ph.is_contiguous() &&
-           ph.scalar_type() == at::kFloat && ph.device() == q.device() && (uintptr_t)ph.data_ptr() % 16 == 0);
-      step = ph.size(0) == 1 ? 0 : (int64_t)T * (d / 2);
+struct QkNorm : torch::autograd::Function<QkNorm> {
+  struct Call {
+    at::Tensor q, k, wq, wk, ph;
+    float eps;
+    int32_t B, T, Hq, Hk, d;
+    int64_t step = 0;
+    Call(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& wq_, const at::Tensor& wk_, const at::Tensor& ph_, double eps_)
+        : q(q_), k(k_), wq(wq_), wk(wk_), ph(ph_), eps((float)eps_) {
+      B = (int32_t)q.size(0); T = (int32_t)q.size(1); Hq = (int32_t)q.size(2); Hk = (int32_t)k.size(2); d = (int32_t)q.size(3);
+      if (ph.defined() && ph.size(0) > 1) step = (int64_t)T * (d / 2);
     }
-    ready(q); ready(k);
-  }
-  void ready(const at::Tensor& t) const { NEED(t.scalar_type() == q.scalar_type() && t.device() == q.device() && in_place(t) && aligned(t, 16)); }
-  const float* weight(const at::Tensor& w) const { return param(w, d, q); }
-  const float* phasors() const { return ph.defined() ? (const float*)ph.data_ptr() : nullptr; }
-};
-// qk_norm_forward(q, k, wq, wk, phasors, eps) -> (yq, yk)
-PyObject* qk_norm_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return guarded(n, 6, [&]() -> PyObject* {
-    const QkNorm c(a);
-    const float eps = (float)real_number(a[5]), *wq = c.weight(c.wq), *wk = c.weight(c.wk);
+    void check() const {
+      NEED(real(q.scalar_type()) && k.scalar_type() == q.scalar_type() && k.device() == q.device() && k.size(0) == B && k.size(1) == T && k.size(3) == d);
+      NEED(d % 8 == 0 && d <= 256 && q.numel() < INT32_MAX && k.numel() < INT32_MAX);
+      NEED(in_place(q) && aligned(q, 16) && in_place(k) && aligned(k, 16));
+      param(wq, d, q); param(wk, d, q);
+      if (ph.defined())
+        NEED(ph.dim() == 4 && (ph.size(0) == 1 || ph.size(0) == B) && ph.size(1) == T && ph.size(2) == d / 2 && ph.size(3) == 2 && ph.is_contiguous() &&
+             ph.scalar_type() == at::kFloat && ph.device() == q.device() && (uintptr_t)ph.data_ptr() % 16 == 0);
+    }
+    static const float* data(const at::Tensor& t) { return t.defined() ? (const float*)t.data_ptr() : nullptr; }
+  };
+  static Tensors run(const Call& c) {
     Place here(c.q);
     const at::Tensor yq = make(c.q.sizes(), c.q, c.q.scalar_type()), yk = make(c.k.sizes(), c.q, c.q.scalar_type());
     const fpb_seq sq = seq(c.q), sk = seq(c.k), oq = seq(yq), ok = seq(yk);
-    const int r = unlocked([&] {
-      return entry.qk_norm_fwd(c.B, c.T, c.Hq, c.Hk, c.d, code(c.q.scalar_type()), eps, wq, wk, c.phasors(), c.step, &sq, &sk, &oq, &ok, here.stream);
-    });
-    return status_or(r, {yq, yk});
-  });
-}
-// qk_norm_backward(q, k, wq, wk, phasors, eps, dyq, dyk, need_wq, need_wk) -> (dq, dk, dwq, dwk)
-PyObject* qk_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return guarded(n, 10, [&]() -> PyObject* {
-    const QkNorm c(a);
-    const float eps = (float)real_number(a[5]), *wq = c.weight(c.wq), *wk = c.weight(c.wk);
-    const at::Tensor dyq = tensor(a[6]), dyk = tensor(a[7]);
-    NEED(dyq.sizes() == c.q.sizes() && dyk.sizes() == c.k.sizes());
-    c.ready(dyq); c.ready(dyk);
+    ran(unlocked([&] {
+      return entry.qk_norm_fwd(c.B, c.T, c.Hq, c.Hk, c.d, code(c.q.scalar_type()), c.eps, c.data(c.wq), c.data(c.wk), c.data(c.ph), c.step, &sq, &sk, &oq,
+                               &ok, here.stream);
+    }));
+    return {yq, yk};
+  }
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const Maybe& wq, const Maybe& wk, const Maybe& ph,
+                               double eps) {
+    variable_list y = run(Call(q, k, or_none(wq), or_none(wk), or_none(ph), eps));
+    ctx->save_for_backward({q, k, or_none(wq), or_none(wk), or_none(ph)});
+    ctx->saved_data["eps"] = eps;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const bool graph = at::GradMode::is_enabled();
+    at::NoGradGuard no_grad;
+    const variable_list v = ctx->get_saved_variables();
+    const Call c(v[0], v[1], v[2], v[3], v[4], ctx->saved_data["eps"].toDouble());
     Place here(c.q);
+    const at::Tensor dyq = readable(g[0]), dyk = readable(g[1]);
     const at::Tensor dq = make(c.q.sizes(), c.q, c.q.scalar_type()), dk = make(c.k.sizes(), c.q, c.q.scalar_type()),
-                     dwq = a[8] == Py_True ? make({c.d}, c.q, at::kFloat) : at::Tensor(), dwk = a[9] == Py_True ? make({c.d}, c.q, at::kFloat) : at::Tensor(),
-                     scratch = make({FPB_QK_NORM_SCRATCH(c.d)}, c.q, at::kByte);
+                     dwq = c.wq.defined() && ctx->needs_input_grad(2) ? make({c.d}, c.q, at::kFloat) : at::Tensor(),
+                     dwk = c.wk.defined() && ctx->needs_input_grad(c.wq.defined() ? 3 : 2) ? make({c.d}, c.q, at::kFloat) : at::Tensor(), scratch = make({FPB_QK_NORM_SCRATCH(c.d)}, c.q, at::kByte);
     const fpb_seq sq = seq(c.q), sk = seq(c.k), gq = seq(dyq), gk = seq(dyk), oq = seq(dq), ok = seq(dk);
-    const int r = unlocked([&] {
-      return entry.qk_norm_bwd(c.B, c.T, c.Hq, c.Hk, c.d, code(c.q.scalar_type()), eps, wq, wk, c.phasors(), c.step, &sq, &sk, &gq, &gk, &oq, &ok,
-                               dwq.defined() ? (float*)dwq.data_ptr() : nullptr, dwk.defined() ? (float*)dwk.data_ptr() : nullptr, scratch.data_ptr(),
-                               here.stream);
-    });
-    return status_or(r, {dq, dk, dwq, dwk});
+    ran_backward(entry.qk_norm_bwd(c.B, c.T, c.Hq, c.Hk, c.d, code(c.q.scalar_type()), c.eps, c.data(c.wq), c.data(c.wk), c.data(c.ph), c.step, &sq, &sk,
+                                   &gq, &gk, &oq, &ok, dwq.defined() ? (float*)dwq.data_ptr() : nullptr, dwk.defined() ? (float*)dwk.data_ptr() : nullptr,
+                                   scratch.data_ptr(), here.stream));
+    return once({dq, dk, dwq, dwk, at::Tensor(), at::Tensor()}, graph);
+  }
+};
+// qk_norm_rotary(q, k, wq, wk, phasors, eps) -> (yq, yk)
+PyObject* qk_norm_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded_call(n, 6, [&]() -> Tensors {
+    const at::Tensor q = tensor(a[0]), k = tensor(a[1]), wq = maybe(a[2]), wk = maybe(a[3]), ph = maybe(a[4]);
+    const double eps = real_number(a[5]);
+    NEED(q.dim() == 4 && k.dim() == 4 && !(ph.defined() && ph.requires_grad()));
+    const QkNorm::Call c(q, k, wq, wk, ph, eps);
+    c.check();
+    return graph_wanted({q, k, wq, wk}) ? QkNorm::apply(q, k, given(wq), given(wk), given(ph), eps) : QkNorm::run(c);
   });
 }
 
+struct Dropout : torch::autograd::Function<Dropout> {
+  static at::Tensor run(const at::Tensor& x, const at::Tensor& res, double p, const at::Tensor& seed, bool backward) {
+    Place here(x);
+    const at::Tensor y = make(x.sizes(), x, x.scalar_type());
+    auto call = [&] {
+      return entry.dropout(x.numel(), code(x.scalar_type()), p, (const int64_t*)seed.data_ptr(), x.data_ptr(), res.defined() ? res.data_ptr() : nullptr,
+                           y.data_ptr(), here.stream);
+    };
+    if (backward) ran_backward(call()); else ran(unlocked(call));
+    return y;
+  }
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const Maybe& res, double p, const at::Tensor& seed) {
+    const at::Tensor y = run(x, or_none(res), p, seed, false);
+    ctx->save_for_backward({seed});
+    ctx->saved_data["residual"] = res.has_value();
+    ctx->saved_data["p"] = p;
+    return {y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const bool graph = at::GradMode::is_enabled();
+    at::NoGradGuard no_grad;
+    const at::Tensor seed = ctx->get_saved_variables()[0];
+    const at::Tensor dx = ctx->needs_input_grad(0) ? run(dense(g[0]), at::Tensor(), ctx->saved_data["p"].toDouble(), seed, true) : at::Tensor();
+    return once({dx, ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(1) ? g[0] : at::Tensor(), at::Tensor(), at::Tensor()}, graph);
+  }
+};
 // dropout(x, residual or None, p, seed) -> (y,)
 PyObject* dropout(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return guarded(n, 4, [&]() -> PyObject* {
+  return guarded_call(n, 4, [&]() -> Tensors {
     const at::Tensor x = tensor(a[0]), res = maybe(a[1]), seed = tensor(a[3]);
     const double p = real_number(a[2]);
     NEED(real(x.scalar_type()) && x.is_contiguous() && p >= 0.0 && p <= 1.0);
     if (res.defined()) NEED(res.scalar_type() == x.scalar_type() && res.sizes() == x.sizes() && res.is_contiguous() && res.device() == x.device());
     NEED(seed.scalar_type() == at::kLong && seed.numel() == 1 && seed.device() == x.device());
-    Place here(x);
-    const at::Tensor y = make(x.sizes(), x, x.scalar_type());
-    const int r = unlocked([&] {
-      return entry.dropout(x.numel(), code(x.scalar_type()), p, (const int64_t*)seed.data_ptr(), x.data_ptr(), res.defined() ? res.data_ptr() : nullptr,
-                           y.data_ptr(), here.stream);
-    });
-    return status_or(r, {y});
+    if (graph_wanted({x, res})) return Dropout::apply(x, given(res), p, seed);
+    return {Dropout::run(x, res, p, seed, false)};
   });
 }
 
@@ -581,87 +676,111 @@ at::Tensor ids(PyObject* o, const at::Tensor& like) {
   NEED(t.scalar_type() == at::kLong && t.is_contiguous() && t.device() == like.device());
   return t;
 }
-// embedding_forward(tokens, weight, scale) -> (y,)
-PyObject* embedding_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return guarded(n, 3, [&]() -> PyObject* {
-    const at::Tensor w = tensor(a[1]), t = ids(a[0], w);
-    const float scale = (float)real_number(a[2]);
-    NEED(real(w.scalar_type()));
-    const int64_t stride = pitch(w), D = w.size(1);
-    NEED(D <= 1 << 20);
-    std::vector<int64_t> shape(t.sizes().begin(), t.sizes().end());
-    shape.push_back(D);
-    Place here(w);
-    const at::Tensor y = make(shape, w, w.scalar_type());
-    const int r = unlocked([&] {
-      return entry.embedding_fwd(t.numel(), w.size(0), (int32_t)D, code(w.scalar_type()), (const int64_t*)t.data_ptr(), w.data_ptr(), stride, scale,
-                                 y.data_ptr(), here.stream);
-    });
-    return status_or(r, {y});
-  });
+std::vector<int64_t> with_last(at::IntArrayRef sizes, int64_t last) {
+  std::vector<int64_t> shape(sizes.begin(), sizes.end());
+  shape.push_back(last);
+  return shape;
 }
-// embedding_backward(tokens, dy (..., D), V, padding, scale) -> (dw,)
-PyObject* embedding_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return guarded(n, 5, [&]() -> PyObject* {
-    const at::Tensor dy = tensor(a[1]), t = ids(a[0], dy);
-    const int64_t V = integer(a[2]), padding = integer(a[3]), N = t.numel(), D = dy.size(-1);
-    const float scale = (float)real_number(a[4]);
-    NEED(real(dy.scalar_type()) && dy.is_contiguous() && dy.numel() == N * D && V > 0 && D <= 1 << 20);
-    Place here(dy);
-    const at::Tensor dw = make({V, D}, dy, dy.scalar_type());
+struct Embedding : torch::autograd::Function<Embedding> {
+  static at::Tensor run(const at::Tensor& t, const at::Tensor& w, double scale) {
+    const int64_t stride = pitch(w), D = w.size(1);
+    Place here(w);
+    const at::Tensor y = make(with_last(t.sizes(), D), w, w.scalar_type());
+    ran(unlocked([&] {
+      return entry.embedding_fwd(t.numel(), w.size(0), (int32_t)D, code(w.scalar_type()), (const int64_t*)t.data_ptr(), w.data_ptr(), stride, (float)scale,
+                                 y.data_ptr(), here.stream);
+    }));
+    return y;
+  }
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& t, const at::Tensor& w, double scale, int64_t padding) {
+    const at::Tensor y = run(t, w, scale);
+    ctx->save_for_backward({t});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding"] = padding;
+    ctx->saved_data["V"] = w.size(0);
+    return {y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const bool graph = at::GradMode::is_enabled();
+    at::NoGradGuard no_grad;
+    const at::Tensor t = ctx->get_saved_variables()[0];
+    const int64_t V = ctx->saved_data["V"].toInt(), D = g[0].size(-1), N = t.numel();
+    Place here(g[0]);
+    const at::Tensor dy = dense(g[0]), dw = make({V, D}, dy, dy.scalar_type());
     const int64_t need = entry.embedding_workspace(N, V, (int32_t)D);
     const at::Tensor scratch = make({need}, dy, at::kByte);
-    const int r = unlocked([&] {
-      return entry.embedding_bwd(N, V, (int32_t)D, code(dy.scalar_type()), (const int64_t*)t.data_ptr(), padding, scale, dy.data_ptr(), D, dw.data_ptr(),
-                                 scratch.data_ptr(), need, here.stream);
-    });
-    return status_or(r, {dw});
+    ran_backward(entry.embedding_bwd(N, V, (int32_t)D, code(dy.scalar_type()), (const int64_t*)t.data_ptr(), ctx->saved_data["padding"].toInt(),
+                                     (float)ctx->saved_data["scale"].toDouble(), dy.data_ptr(), D, dw.data_ptr(), scratch.data_ptr(), need, here.stream));
+    return once({at::Tensor(), dw, at::Tensor(), at::Tensor()}, graph);
+  }
+};
+// embedding(tokens, weight, scale, padding) -> (y,)
+PyObject* embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded_call(n, 4, [&]() -> Tensors {
+    const at::Tensor w = tensor(a[1]), t = ids(a[0], w);
+    const double scale = real_number(a[2]);
+    const int64_t padding = integer(a[3]);
+    NEED(real(w.scalar_type()) && w.dim() == 2 && w.size(1) <= 1 << 20);
+    pitch(w);
+    if (graph_wanted({w})) return Embedding::apply(t, w, scale, padding);
+    return {Embedding::run(t, w, scale)};
   });
 }
 
-// scores_forward(logits (..., V), tokens (...), top) -> (logprob, entropy, stats, top_logprob or None, top_tokens or None)
-PyObject* scores_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return guarded(n, 3, [&]() -> PyObject* {
-    const at::Tensor z = tensor(a[0]), t = ids(a[1], z);
-    const int64_t top = integer(a[2]);
-    NEED(z.dim() >= 1 && t.sizes() == z.sizes().slice(0, z.dim() - 1) && real(z.scalar_type()) && (z.is_contiguous() || z.dim() == 2));
-    const int64_t V = z.size(-1), rows = t.numel(), stride = z.is_contiguous() ? V : pitch(z);
-    NEED(top >= 0 && top <= FPB_MAX_TOP && top <= V && V <= 1 << 30);
+struct Scores : torch::autograd::Function<Scores> {
+  static int64_t stride(const at::Tensor& z) { return z.is_contiguous() ? z.size(-1) : pitch(z); }
+  // logprob, entropy, top_logprob, top_tokens (undefined without alternatives), stats
+  static Tensors run(const at::Tensor& z, const at::Tensor& t, int64_t top) {
+    const int64_t V = z.size(-1), rows = t.numel(), pitch_z = stride(z);
     Place here(z);
     const at::Tensor lp = make(t.sizes(), z, at::kFloat), h = make(t.sizes(), z, at::kFloat), stats = make({rows, 2}, z, at::kFloat);
     at::Tensor tl, tt;
-    if (top) {
-      std::vector<int64_t> shape(t.sizes().begin(), t.sizes().end());
-      shape.push_back(top);
-      tl = make(shape, z, at::kFloat);
-      tt = make(shape, z, at::kLong);
-    }
-    const int r = unlocked([&] {
-      return entry.scores_fwd(rows, (int32_t)V, code(z.scalar_type()), (int32_t)top, z.data_ptr(), stride, (const int64_t*)t.data_ptr(), (float*)lp.data_ptr(),
+    if (top) { tl = make(with_last(t.sizes(), top), z, at::kFloat); tt = make(with_last(t.sizes(), top), z, at::kLong); }
+    ran(unlocked([&] {
+      return entry.scores_fwd(rows, (int32_t)V, code(z.scalar_type()), (int32_t)top, z.data_ptr(), pitch_z, (const int64_t*)t.data_ptr(), (float*)lp.data_ptr(),
                               (float*)h.data_ptr(), (float*)stats.data_ptr(), top ? (float*)tl.data_ptr() : nullptr,
                               top ? (int64_t*)tt.data_ptr() : nullptr, here.stream);
-    });
-    return status_or(r, {lp, h, stats, tl, tt});
-  });
-}
-// scores_backward(logits, tokens, entropy, stats, top_tokens or None, g_logprob, g_entropy, g_top (each or None)) -> (d,)
-PyObject* scores_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return guarded(n, 8, [&]() -> PyObject* {
-    const at::Tensor z = tensor(a[0]), t = ids(a[1], z), h = tensor(a[2]), stats = tensor(a[3]), tt = maybe(a[4]);
-    const at::Tensor g[3] = {maybe(a[5]), maybe(a[6]), maybe(a[7])};
-    NEED(z.is_contiguous() || z.dim() == 2);
-    const int64_t V = z.size(-1), rows = t.numel(), stride = z.is_contiguous() ? V : pitch(z), top = tt.defined() ? tt.size(-1) : 0;
-    for (int i = 0; i < 3; ++i)
-      if (g[i].defined())
-        NEED(g[i].scalar_type() == at::kFloat && g[i].is_contiguous() && g[i].device() == z.device() && g[i].numel() == (i < 2 ? rows : rows * top));
+    }));
+    return {lp, h, tl, tt, stats};
+  }
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& z, const at::Tensor& t, int64_t top) {
+    Tensors r = run(z, t, top);
+    ctx->save_for_backward({z, t, r[1], r[4], r[3]});
+    ctx->set_materialize_grads(false);
+    if (top) ctx->mark_non_differentiable({r[3]});
+    r.resize(top ? 4 : 2);
+    return r;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const bool graph = at::GradMode::is_enabled();
+    at::NoGradGuard no_grad;
+    const variable_list v = ctx->get_saved_variables();
+    const at::Tensor &z = v[0], &t = v[1], &tt = v[4];
+    const int64_t V = z.size(-1), rows = t.numel(), top = tt.defined() ? tt.size(-1) : 0;
+    at::Tensor gs[3];
+    for (size_t i = 0; i < 3 && i < g.size(); ++i)
+      if (g[i].defined()) gs[i] = g[i].contiguous();
+    if (!gs[0].defined() && !gs[1].defined() && !gs[2].defined()) return {at::Tensor(), at::Tensor(), at::Tensor()};
     Place here(z);
     const at::Tensor d = make(z.sizes(), z, z.scalar_type());
     auto at = [](const at::Tensor& x) { return x.defined() ? (const float*)x.data_ptr() : nullptr; };
-    const int r = unlocked([&] {
-      return entry.scores_bwd(rows, (int32_t)V, code(z.scalar_type()), (int32_t)top, z.data_ptr(), stride, (const int64_t*)t.data_ptr(), at(h), at(stats),
-                              tt.defined() ? (const int64_t*)tt.data_ptr() : nullptr, at(g[0]), at(g[1]), at(g[2]), d.data_ptr(), V, here.stream);
-    });
-    return status_or(r, {d});
+    ran_backward(entry.scores_bwd(rows, (int32_t)V, code(z.scalar_type()), (int32_t)top, z.data_ptr(), stride(z), (const int64_t*)t.data_ptr(), at(v[2]),
+                                  at(v[3]), tt.defined() ? (const int64_t*)tt.data_ptr() : nullptr, at(gs[0]), at(gs[1]), at(gs[2]), d.data_ptr(), V,
+                                  here.stream));
+    return once({d, at::Tensor(), at::Tensor()}, graph);
+  }
+};
+// token_scores(logits (..., V), tokens (...), top) -> (logprob, entropy, top_logprob or None, top_tokens or None)
+PyObject* token_scores(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded_call(n, 3, [&]() -> Tensors {
+    const at::Tensor z = tensor(a[0]), t = ids(a[1], z);
+    const int64_t top = integer(a[2]);
+    NEED(z.dim() >= 1 && t.sizes() == z.sizes().slice(0, z.dim() - 1) && real(z.scalar_type()) && (z.is_contiguous() || z.dim() == 2));
+    NEED(top >= 0 && top <= FPB_MAX_TOP && top <= z.size(-1) && z.size(-1) <= 1 << 30);
+    Scores::stride(z);
+    Tensors r = graph_wanted({z}) ? Scores::apply(z, t, top) : Scores::run(z, t, top);
+    r.resize(4);
+    return r;
   });
 }
 
@@ -705,8 +824,8 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(step), FAST(forward), FAST(backward), FAST(suffix_forward), FAST(suffix_backward), FAST(rotary), FAST(gate_forward),
-                         FAST(gate_backward), FAST(norm_forward), FAST(norm_backward), FAST(column_sums), FAST(qk_norm_forward), FAST(qk_norm_backward),
-                         FAST(dropout), FAST(embedding_forward), FAST(embedding_backward), FAST(scores_forward), FAST(scores_backward), FAST(address), FAST(wanted), FAST(bind), {nullptr, nullptr, 0, nullptr}};
+                         FAST(gate_backward), FAST(norm_forward), FAST(norm_backward), FAST(column_sums), FAST(qk_norm_rotary), FAST(dropout),
+                         FAST(embedding), FAST(token_scores), FAST(address), FAST(wanted), FAST(bind), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "fpb_fast_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -10,7 +10,7 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from flash_pop_b200 import _lib
-from flash_pop_b200.layer_ops import _OK_DTYPES, _ptr, no_graph
+from flash_pop_b200.layer_ops import _OK_DTYPES, _ptr
 
 MAX_TOP = 32
 
@@ -33,11 +33,6 @@ def _pitch(t: Tensor) -> int:
 class Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, tokens, weight, scale, padding):
-        fast = _lib.result(_lib.native().embedding_forward(tokens, weight, scale))
-        if fast is not None:
-            ctx.save_for_backward(tokens)
-            ctx.of = *weight.shape, weight.dtype, scale, padding
-            return fast[0]
         _check_embedding(tokens, weight)
         tokens = tokens.to(torch.int64)
         w, ids = _matrix(weight), tokens.contiguous()
@@ -56,10 +51,6 @@ class Embedding(torch.autograd.Function):
     def backward(ctx, dy):
         (ids,) = ctx.saved_tensors
         V, D, dtype, scale, padding = ctx.of
-        if dy.dtype == dtype:
-            fast = _lib.result(_lib.native().embedding_backward(ids, dy, V, padding, scale))
-            if fast is not None:
-                return None, fast[0], None, None
         N = ids.numel()
         dy = _matrix(dy.to(dtype).reshape(N, D))
         dw = torch.empty((V, D), device=dy.device, dtype=dtype)
@@ -90,10 +81,9 @@ def embedding(tokens: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: O
         if not -V <= padding_idx < V:
             raise ValueError(f"padding_idx {padding_idx} outside a table of {V} rows")
         padding = padding_idx % V
-    if no_graph(weight):
-        fast = _lib.result(_lib.native().embedding_forward(tokens, weight, scale))
-        if fast is not None:
-            return fast[0]
+    fast = _lib.result(_lib.native().embedding(tokens, weight, scale, padding))
+    if fast is not None:
+        return fast[0]
     return Embedding.apply(tokens, weight, scale, padding)
 
 
@@ -121,21 +111,17 @@ def _check_scores(logits: Tensor, tokens: Tensor, top: int) -> None:
 class _TokenScores(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top):
-        fast = _lib.result(_lib.native().scores_forward(logits, tokens, top))
-        if fast is not None:
-            logprob, entropy, stats, top_logprob, top_tokens = fast
-        else:
-            _check_scores(logits, tokens, top)
-            shape, V = tokens.shape, logits.size(-1)
-            tokens, z = tokens.to(torch.int64).reshape(-1).contiguous(), _matrix(logits.reshape(-1, V))
-            rows, dev = tokens.numel(), z.device
-            new = lambda *extra, dtype=torch.float32: torch.empty((*shape, *extra), device=dev, dtype=dtype)
-            logprob, entropy, stats = new(), new(), torch.empty((rows, 2), device=dev, dtype=torch.float32)
-            top_logprob, top_tokens = (new(top), new(top, dtype=torch.int64)) if top else (None, None)
-            with torch.cuda.device(dev):
-                _lib.check(_lib.lib().fpb_token_scores_fwd(rows, V, _lib.dtype_code(z), top, _ptr(z), _pitch(z), _ptr(tokens), _ptr(logprob),
-                                                           _ptr(entropy), _ptr(stats), _ptr(top_logprob), _ptr(top_tokens), _lib.stream_ptr(dev)))
-            logits = z.view(logits.shape) if z.is_contiguous() else logits
+        _check_scores(logits, tokens, top)
+        shape, V = tokens.shape, logits.size(-1)
+        tokens, z = tokens.to(torch.int64).reshape(-1).contiguous(), _matrix(logits.reshape(-1, V))
+        rows, dev = tokens.numel(), z.device
+        new = lambda *extra, dtype=torch.float32: torch.empty((*shape, *extra), device=dev, dtype=dtype)
+        logprob, entropy, stats = new(), new(), torch.empty((rows, 2), device=dev, dtype=torch.float32)
+        top_logprob, top_tokens = (new(top), new(top, dtype=torch.int64)) if top else (None, None)
+        with torch.cuda.device(dev):
+            _lib.check(_lib.lib().fpb_token_scores_fwd(rows, V, _lib.dtype_code(z), top, _ptr(z), _pitch(z), _ptr(tokens), _ptr(logprob),
+                                                       _ptr(entropy), _ptr(stats), _ptr(top_logprob), _ptr(top_tokens), _lib.stream_ptr(dev)))
+        logits = z.view(logits.shape) if z.is_contiguous() else logits
         ctx.save_for_backward(logits, tokens, entropy, stats, top_tokens)
         ctx.set_materialize_grads(False)
         if top:
@@ -148,9 +134,6 @@ class _TokenScores(torch.autograd.Function):
         logits, tokens, entropy, stats, top_tokens = ctx.saved_tensors
         if g_logprob is None and g_entropy is None and g_top is None:
             return None, None, None
-        fast = _lib.result(_lib.native().scores_backward(logits, tokens, entropy, stats, top_tokens, g_logprob, g_entropy, g_top))
-        if fast is not None:
-            return fast[0], None, None
         V = logits.size(-1)
         z = _matrix(logits.reshape(-1, V))
         rows = z.size(0)
@@ -168,8 +151,7 @@ def token_scores(logits: Tensor, tokens: Tensor, top: int = 0) -> TokenScores:
     tokens with their log probabilities, equal logits by index; fp32 arithmetic, one read of the logits.  All but the indices are
     differentiable (one more read and one write).  A token outside [0, V) has the log probability 0 and sends no gradient
     (`cross_entropy`'s rule).  A row of -inf only gives -inf, entropy 0 and no gradient; NaN or +inf in a row make its numbers NaN."""
-    if no_graph(logits):
-        fast = _lib.result(_lib.native().scores_forward(logits, tokens, top))
-        if fast is not None:
-            return TokenScores(fast[0], fast[1], fast[3], fast[4])
+    fast = _lib.result(_lib.native().token_scores(logits, tokens, top))
+    if fast is not None:
+        return TokenScores(*fast)
     return TokenScores(*_TokenScores.apply(logits, tokens, top))

@@ -48,23 +48,58 @@ def test_ordinary_calls_are_taken_and_others_left():
     g = torch.Generator(device="cuda").manual_seed(1)
     rnd = lambda *s, t=BF: torch.randn(*s, generator=g, device="cuda").to(t)
     q, w, ph = rnd(2, 3, 4, 64), rnd(64, t=torch.float32), rnd(1, 3, 32, 2, t=torch.float32)
-    assert n.qk_norm_forward(q, q, w, None, ph, 1e-6) is not None and n.qk_norm_backward(q, q, w, None, ph, 1e-6, q, q, True, False)[3] is None
+    assert n.qk_norm_rotary(q, q, w, None, ph, 1e-6) is not None
     for bad in ((q, q, w[:32], None, ph, 1e-6), (q, q.float(), w, None, ph, 1e-6), (q, q, w.to(BF), None, ph, 1e-6), (q, q, w, None, ph[:, :2], 1e-6),
                 (q, q, w, None, ph, 1), (q.transpose(0, 1), q, w, None, ph, 1e-6), (q[..., :60], q[..., :60], None, None, None, 1e-6)):
-        assert n.qk_norm_forward(*bad) is None
+        assert n.qk_norm_rotary(*bad) is None
     x, seed = rnd(5, 7), torch.tensor([1], device="cuda")
     assert n.dropout(x, x, 0.5, seed) is not None
     for bad in ((x, x[:4], 0.5, seed), (x, x.float(), 0.5, seed), (x, None, 1.5, seed), (x, None, 0.5, seed.int()), (x, None, 0.5, seed.cpu()),
                 (x.t(), None, 0.5, seed), (x.half(), None, 0.5, seed), (x, None, float("nan"), seed)):
         assert n.dropout(*bad) is None
     t = torch.randint(0, 5, (4,), device="cuda")
-    assert n.embedding_forward(t, x, 1.0) is not None and n.embedding_backward(t, x[:4], 9, -1, 1.0) is not None
-    for bad in ((t.int(), x, 1.0), (t, x.t(), 1.0), (t, x.half(), 1.0), (t[:0], x, 1.0), (t.cpu(), x, 1.0), (t, x, 1)):
-        assert n.embedding_forward(*bad) is None
-    assert n.embedding_backward(t, x, 9, -1, 1.0) is None and n.embedding_backward(t, x[:4].t().contiguous().t(), 9, -1, 1.0) is None
-    assert n.scores_forward(x[:4], t, 3) is not None
+    assert n.embedding(t, x, 1.0, -1) is not None
+    for bad in ((t.int(), x, 1.0, -1), (t, x.t(), 1.0, -1), (t, x.half(), 1.0, -1), (t[:0], x, 1.0, -1), (t.cpu(), x, 1.0, -1), (t, x, 1, -1), (t, x, 1.0, None)):
+        assert n.embedding(*bad) is None
+    assert n.token_scores(x[:4], t, 3) is not None
     for bad in ((x, t, 3), (x[:4], t, 8), (x[:4], t, 33), (x[:4], t, -1), (x[:4].half(), t, 0), (x[:4], t.int(), 0), (rnd(4, 2, 7)[:, 0], t[:3], 0)):
-        assert n.scores_forward(*bad) is None
+        assert n.token_scores(*bad) is None
+
+
+@pytest.mark.parametrize("name", ["qk_norm_rotary", "dropout", "embedding", "token_scores"])
+@pytest.mark.parametrize("fast", [True, False])
+def test_partial_gradients_strided_gradients_and_second_ones(name, fast, monkeypatch):
+    from flash_pop_b200 import _lib
+    if not fast:
+        monkeypatch.setattr(_lib, "native", lambda: _lib._Declines())
+    inputs, call = _calls()[name]
+    leaves = [t.detach().clone().requires_grad_(True) for t in inputs]
+    ends = [t for t in call(*leaves) if t is not None and t.is_floating_point()]
+    want = torch.autograd.grad(ends, leaves, [torch.ones_like(t) for t in ends], retain_graph=True)
+    for i, leaf in enumerate(leaves):                              # one input's alone: the others need none
+        (got,) = torch.autograd.grad(ends, [leaf], [torch.ones_like(t) for t in ends], retain_graph=True)
+        assert torch.equal(got, want[i])
+    got = torch.autograd.grad(ends, leaves, [torch.ones(1, device="cuda", dtype=t.dtype).expand(t.shape) for t in ends], retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))       # expanded gradients, which no kernel reads in place
+    odd = [torch.ones(*t.shape[:-1], t.shape[-1] + 1, device="cuda", dtype=t.dtype)[..., 1:] for t in ends]
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(ends, leaves, odd, retain_graph=True), want))
+    few = [t.detach().requires_grad_(i == 0) for i, t in enumerate(leaves)]
+    out = [t for t in call(*few) if t is not None and t.is_floating_point()]
+    assert torch.equal(torch.autograd.grad(out, few[:1], [torch.ones_like(t) for t in out])[0], want[0])
+    gs = [torch.ones_like(t, requires_grad=True) for t in ends]
+    once = torch.autograd.grad(ends, leaves, gs, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(once, want))
+    with pytest.raises(RuntimeError, match="twice"):
+        once[0].float().pow(2).sum().backward()
+
+
+def test_saved_tensors_that_change_raise():
+    from flash_pop_b200 import layer_ops
+    x, seed = torch.randn(50, device="cuda", requires_grad=True), torch.tensor([3], device="cuda")
+    y = layer_ops.dropout(x, 0.5, seed)
+    seed.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y.sum(), [x])
 
 
 def test_forward_mode_gradients_are_not_dropped():
