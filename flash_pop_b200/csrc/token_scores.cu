@@ -376,8 +376,9 @@ template <int NT> __device__ __forceinline__ uint32_t part_maxima(float most, bo
   return few ? sorted : merge_sorted(sorted, sort_warp(group[32 + lane]));
 }
 
-// The elements of a thread's vectors that reach the bound join the candidates, as far as there is room.
-template <typename T, int NT, int N> __device__ __forceinline__ void push(const Row<T>& row, const Vectors<N>& from, int first, int end, float bound,
+// The elements of a thread's vectors that reach the bound join the candidates, as far as there is room.  STRICT: those at a bound
+// as low as a mask's value do not.
+template <typename T, int NT, bool STRICT, int N> __device__ __forceinline__ void push(const Row<T>& row, const Vectors<N>& from, int first, int end, float bound,
                                                                          Shared<NT / 32>& sh) {
 #pragma unroll
   for (int j = 0; j < N; ++j) {
@@ -386,7 +387,7 @@ template <typename T, int NT, int N> __device__ __forceinline__ void push(const 
 #pragma unroll
     for (int e = 0; e < Row<T>::E; ++e) {
       const float z = element<T>(from.r[j], e);
-      if (z < bound) continue;
+      if (z < bound || (STRICT && bound < SMALLEST && z == bound)) continue;
       const int at = atomicAdd(&sh.found, 1);
       if (at < CANDIDATES) sh.candidate[at] = rank_key(z, row.index(v, e));
     }
@@ -408,7 +409,7 @@ template <typename T, int NT> __device__ __noinline__ void careful_candidates(co
     if (NT == 32) __syncthreads();
     least = max(least, __shfl_sync(ALL, sorted, top - 1));
     const float bound = value_of(least);
-    if (!(most < bound)) push<T, NT>(row, tile, first, end, bound, sh);
+    if (!(most < bound)) push<T, NT, false>(row, tile, first, end, bound, sh);
     __syncthreads();
     if (sh.found > CANDIDATES) {
       // no room: the `top` best that earlier tiles left, and this tile's
@@ -469,9 +470,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) scores_kernel(const __grid_cons
         parts = i == 0 ? sorted : merge_sorted(parts, sorted);
         bound = value_of(__shfl_sync(ALL, parts, p.top - 1));
       }
-      if (!(most < bound)) {
+      // (a bound as low as a mask's value: only what is above it, the rest of the choice is made below)
+      if (bound < SMALLEST ? !(most <= bound) : !(most < bound)) {
         if (end - begin <= N * NT) {                 // (all there is: nothing to wait for)
-          push<T, NT>(row, now, first, end, bound, sh);
+          push<T, NT, true>(row, now, first, end, bound, sh);
         } else {
           const int at = atomicAdd(&sh.records, 1);
           if (at < RECORDS) sh.record[at] = make_uint2(order_of(most), (uint32_t)(first + threadIdx.x));
@@ -484,6 +486,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) scores_kernel(const __grid_cons
   if constexpr (TOP) {
     __syncthreads();
     const int records = sh.records;
+    const bool masked = bound < SMALLEST;
     if (records <= RECORDS) {
       const uint32_t least = bound == -INFINITY ? 0 : order_of(bound);
       for (int q = warp; q < records; q += WARPS) {
@@ -491,13 +494,26 @@ __global__ void __launch_bounds__(NT, 1024 / NT) scores_kernel(const __grid_cons
         const int v = (int)at.y + lane / E * NT;
         if (at.x < least || lane >= N * E || v >= end) continue;
         const float z = to_float(row.z[row.index(v, lane % E)]);
-        if (z < bound) continue;
+        if (z < bound || (masked && z == bound)) continue;
         const int to = atomicAdd(&sh.found, 1);
         if (to < CANDIDATES) sh.candidate[to] = rank_key(z, row.index(v, lane % E));
       }
     }
     __syncthreads();
-    if (records > RECORDS || sh.found > CANDIDATES) careful_candidates<T, NT>(row, begin, end, p.top, sh);
+    int found = sh.found;
+    if (masked && records <= RECORDS && found < p.top) {
+      // A row of masked elements but for a few: of the first elements at the bound there are enough, as a rule.
+      __syncthreads();
+      const int there = (end - begin) * E;
+      for (int i = threadIdx.x; i < 4 * p.top && i < there; i += NT) {
+        const float z = to_float(row.z[row.index(begin, i)]);
+        if (z == bound) sh.candidate[atomicAdd(&sh.found, 1)] = rank_key(z, row.index(begin, i));
+      }
+      __syncthreads();
+      found = sh.found;
+      if (found < p.top && there > 4 * p.top) found = CANDIDATES + 1;
+    }
+    if (records > RECORDS || found > CANDIDATES) careful_candidates<T, NT>(row, begin, end, p.top, sh);
     if (has_edge && !(edge < bound)) sh.candidate[atomicAdd(&sh.found, 1)] = rank_key(edge, row.edge(threadIdx.x));
     __syncthreads();
     kept = sh.found;
