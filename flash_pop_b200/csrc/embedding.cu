@@ -3,6 +3,8 @@
 // An id outside the table has a zero row and no part in the gradient, and so has the padding id in the gradient.
 // Bound by HBM: forward reads the rows in use and writes N rows, backward reads N rows and writes the dense table.  The
 // gradient has to put the ids in order first (else rows of one id are added by atomics, in another order every time).
+#include <atomic>
+
 #include "fpb_common.cuh"
 #include "vec_io.cuh"
 
@@ -20,24 +22,41 @@ struct LookupParams {
   float scale;
 };
 
+// Threads share a row, units apart; each has ROWS rows in flight.
+constexpr int ROWS = 4;
+
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(THREADS) lookup_kernel(const __grid_constant__ LookupParams p) {
-  const int per = 1 << p.log_threads, lane = threadIdx.x & (per - 1);
-  const int64_t n = (int64_t)blockIdx.x * (THREADS >> p.log_threads) + (threadIdx.x >> p.log_threads);
-  if (n >= p.N) return;
-  const int64_t t = p.tokens[n];
-  const bool inside = t >= 0 && t < p.V;
-  const T* w = (const T*)p.weight + (inside ? t : 0) * p.w_stride;
-  T* y = (T*)p.y + n * p.D;
-  for (int u = lane; u < p.units; u += per) {
-    if constexpr (WIDE) {
-      float f[8];
-      load8(w + u * 8, f);
+  const int per = 1 << p.log_threads, lane = threadIdx.x & (per - 1), groups = THREADS >> p.log_threads;
+  const int64_t n0 = (int64_t)blockIdx.x * groups * ROWS + (threadIdx.x >> p.log_threads);
+  if (n0 >= p.N) return;
+  int64_t token[ROWS];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = inside ? f[e] * p.scale : 0.0f;
-      store8(y + u * 8, f);
-    } else {
-      y[u] = from_float<T>(inside ? to_float(w[u]) * p.scale : 0.0f);
+  for (int i = 0; i < ROWS; ++i) token[i] = n0 + i * groups < p.N ? p.tokens[n0 + i * groups] : -1;
+  for (int u = lane; u < p.units; u += per) {
+    Raw8<T> row[WIDE ? ROWS : 1];
+    T single[WIDE ? 1 : ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const bool inside = token[i] >= 0 && token[i] < p.V;
+      const T* w = (const T*)p.weight + (inside ? token[i] : 0) * p.w_stride;
+      if constexpr (WIDE) read8(w + u * 8, row[i]); else single[i] = w[u];
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int64_t n = n0 + i * groups;
+      if (n >= p.N) break;
+      const bool inside = token[i] >= 0 && token[i] < p.V;
+      T* y = (T*)p.y + n * p.D;
+      if constexpr (WIDE) {
+        float f[8];
+        unpack8(row[i], f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = inside ? f[e] * p.scale : 0.0f;
+        store8(y + u * 8, f);
+      } else {
+        y[u] = from_float<T>(inside ? to_float(single[i]) * p.scale : 0.0f);
+      }
     }
   }
 }
@@ -45,7 +64,9 @@ __global__ void __launch_bounds__(THREADS) lookup_kernel(const __grid_constant__
 // ---- gradient: ids in order -----------------------------------------------------------------------------------------
 // The ids are brought into order with their positions by a stable radix sort, so that the rows of one id follow one another in
 // the order of their positions.  An id without a part (outside the table, or the padding) counts as V and comes last.
-constexpr int RADIX_BITS = 8, RADIX = 1 << RADIX_BITS, SORT_WARPS = THREADS / 32, PER_THREAD = 16, SUB = THREADS * PER_THREAD, MAX_TILES = 256;
+constexpr int RADIX_BITS = 8, RADIX = 1 << RADIX_BITS, PER_THREAD = 8, MAX_TILES = 256;
+constexpr int TILE_THREADS = 512, SUB = TILE_THREADS * PER_THREAD;              // of the sort by many CTAs
+constexpr int ONE_THREADS = 1024, ONE = ONE_THREADS * PER_THREAD;               // of the sort by one CTA
 
 struct SortParams {
   const int64_t* tokens;       // first pass: the ids as the caller gave them
@@ -65,146 +86,181 @@ __device__ __forceinline__ uint2 entry(const SortParams& p, int64_t n) {
 }
 __device__ __forceinline__ uint32_t digit(const SortParams& p, uint32_t key, int shift) { return (key >> shift) & ((1u << p.bits) - 1u); }
 
-__device__ void clear_table(const SortParams& p, int cta, int ctas) {
-  for (int64_t i = (int64_t)cta * THREADS + threadIdx.x; i < p.zero_units; i += (int64_t)ctas * THREADS) p.zero[i] = make_uint4(0, 0, 0, 0);
-  for (int64_t i = (int64_t)cta * THREADS + threadIdx.x; i < p.zero_elements; i += (int64_t)ctas * THREADS) {
+template <int T> __device__ void clear_table(const SortParams& p, int cta, int ctas) {
+  for (int64_t i = (int64_t)cta * T + threadIdx.x; i < p.zero_units; i += (int64_t)ctas * T) p.zero[i] = make_uint4(0, 0, 0, 0);
+  for (int64_t i = (int64_t)cta * T + threadIdx.x; i < p.zero_elements; i += (int64_t)ctas * T) {
     if (p.element == 2) ((uint16_t*)p.zero_tail)[i] = 0; else ((uint32_t*)p.zero_tail)[i] = 0;
   }
 }
 
 // How often each digit stands in each tile.  The CTAs behind the tiles' clear the table meanwhile (first pass): the sort leaves
 // the memory idle.
-__global__ void __launch_bounds__(THREADS) digit_counts_kernel(const __grid_constant__ SortParams p) {
+__global__ void __launch_bounds__(TILE_THREADS) digit_counts_kernel(const __grid_constant__ SortParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if ((int)blockIdx.x >= p.tiles) {
-    clear_table(p, blockIdx.x - p.tiles, gridDim.x - p.tiles);
+    clear_table<TILE_THREADS>(p, blockIdx.x - p.tiles, gridDim.x - p.tiles);
     return;
   }
   __shared__ uint32_t count[RADIX];
-  count[threadIdx.x] = 0;
+  if (threadIdx.x < RADIX) count[threadIdx.x] = 0;
   __syncthreads();
   const int64_t n0 = (int64_t)blockIdx.x * p.subs * SUB, n1 = min(n0 + (int64_t)p.subs * SUB, p.N);
-#pragma unroll 4
-  for (int64_t n = n0 + threadIdx.x; n < n1; n += THREADS) atomicAdd(&count[digit(p, entry(p, n).x, p.shift)], 1u);
+  for (int64_t n = n0 + threadIdx.x; n < n1; n += SUB) {
+    // (entries behind the end repeat the last one and are not counted: a load behind a branch would wait for the one before)
+    uint32_t d[PER_THREAD];
+#pragma unroll
+    for (int i = 0; i < PER_THREAD; ++i) d[i] = digit(p, entry(p, min(n + i * TILE_THREADS, n1 - 1)).x, p.shift);
+#pragma unroll
+    for (int i = 0; i < PER_THREAD; ++i)
+      if (n + i * TILE_THREADS < n1) atomicAdd(&count[d[i]], 1u);
+  }
   __syncthreads();
-  p.counts[blockIdx.x * RADIX + threadIdx.x] = count[threadIdx.x];
+  if (threadIdx.x < RADIX) p.counts[blockIdx.x * RADIX + threadIdx.x] = count[threadIdx.x];
 }
 
-// sum over the threads before this one
-__device__ uint32_t block_scan(uint32_t v, uint32_t (&sums)[SORT_WARPS]) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t x = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
-  if (lane == 31) sums[warp] = x;
-  __syncthreads();
-  for (int w = 0; w < warp; ++w) x += sums[w];
-  return x - v;
-}
+// The places of a CTA's T * PER_THREAD entries when they are put in order of one digit, equal digits in the order they stand in:
+// each warp has 32 * PER_THREAD consecutive ones, lane after lane.
+template <int T> struct Order {
+  static constexpr int WARPS = T / 32;
+  uint32_t before[WARPS][RADIX], sums[RADIX / 32];
 
-// Ranks of a CTA's SUB entries among those of the same digit, in their order: each warp has 32 * PER_THREAD consecutive ones.
-// Leaves in `before` what stands of the digit in the warp so far.
-__device__ __forceinline__ void warp_ranks(const uint32_t (&d)[PER_THREAD], uint32_t (&rank)[PER_THREAD], uint32_t* before) {
-  const unsigned lower = (1u << (threadIdx.x & 31)) - 1u;
-#pragma unroll
-  for (int i = 0; i < PER_THREAD; ++i) {
-    const unsigned same = __match_any_sync(0xffffffffu, d[i]);
-    const bool real = d[i] < RADIX;
-    if (real) rank[i] = before[d[i]] + __popc(same & lower);
-    __syncwarp();
-    if (real && (same & lower) == 0) before[d[i]] += __popc(same);
-    __syncwarp();
+  __device__ void clear() {
+    for (int i = threadIdx.x; i < WARPS * RADIX; i += T) (&before[0][0])[i] = 0;
+    __syncthreads();
   }
-}
+  // Ranks of a warp's entries among those of the same digit; leaves in `before` how many of each digit the warp has.  Which lanes share a digit is
+  // found by a ballot for each of its bits.  One barrier.
+  __device__ void rank(const uint32_t (&d)[PER_THREAD], uint32_t (&r)[PER_THREAD]) {
+    const unsigned lower = (1u << (threadIdx.x & 31)) - 1u;
+    uint32_t* mine = before[threadIdx.x >> 5];
+    unsigned same[PER_THREAD];
+#pragma unroll
+    for (int i = 0; i < PER_THREAD; ++i) {
+      same[i] = __ballot_sync(0xffffffffu, d[i] < RADIX);
+#pragma unroll
+      for (int b = 0; b < RADIX_BITS; ++b) {
+        const bool one = d[i] >> b & 1u;
+        const unsigned ones = __ballot_sync(0xffffffffu, one);
+        same[i] &= one ? ones : ~ones;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < PER_THREAD; ++i) {
+      const bool real = d[i] < RADIX;
+      if (real) r[i] = mine[d[i]] + __popc(same[i] & lower);
+      __syncwarp();
+      if (real && (same[i] & lower) == 0) mine[d[i]] += __popc(same[i]);
+      __syncwarp();
+    }
+    __syncthreads();
+  }
+  // sum over the digits before thread's (threads below RADIX); one barrier
+  __device__ uint32_t scan(uint32_t v) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31 && warp < RADIX / 32) sums[warp] = x;
+    __syncthreads();
+    for (int w = 0; w < warp && w < RADIX / 32; ++w) x += sums[w];
+    return x - v;
+  }
+  // counts of the warps -> where each warp's part of a digit begins; base: where the digit does, moved on.  One barrier.
+  __device__ void place(uint32_t& base) {
+    if (threadIdx.x < RADIX) {
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const uint32_t c = before[w][threadIdx.x];
+        before[w][threadIdx.x] = base;
+        base += c;
+      }
+    }
+    __syncthreads();
+  }
+  __device__ uint32_t at(uint32_t d, uint32_t r) const { return before[threadIdx.x >> 5][d] + r; }
+};
 
 // Every entry to its place: behind all smaller digits, and behind the same digit in earlier tiles, warps and lanes.
-__global__ void __launch_bounds__(THREADS) scatter_kernel(const __grid_constant__ SortParams p) {
-  __shared__ uint32_t before[SORT_WARPS][RADIX], sums[SORT_WARPS];
+__global__ void __launch_bounds__(TILE_THREADS) scatter_kernel(const __grid_constant__ SortParams p) {
+  __shared__ Order<TILE_THREADS> order;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   uint32_t mine = 0, all = 0;                                      // of digit threadIdx.x, in earlier tiles and in all
-#pragma unroll 8
-  for (int t = 0; t < p.tiles; ++t) {
-    const uint32_t c = p.counts[t * RADIX + threadIdx.x];
-    all += c;
-    if (t < (int)blockIdx.x) mine += c;
+  if (threadIdx.x < RADIX) {
+    for (int t0 = 0; t0 < p.tiles; t0 += 16) {
+      uint32_t c[16];
+#pragma unroll
+      for (int t = 0; t < 16; ++t) c[t] = p.counts[min(t0 + t, p.tiles - 1) * RADIX + threadIdx.x];
+#pragma unroll
+      for (int t = 0; t < 16; ++t) {
+        if (t0 + t < p.tiles) all += c[t];
+        if (t0 + t < (int)blockIdx.x) mine += c[t];
+      }
+    }
   }
-  uint32_t base = block_scan(all, sums) + mine;
+  uint32_t base = order.scan(all) + mine;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int s = 0; s < p.subs; ++s) {
     const int64_t n0 = ((int64_t)blockIdx.x * p.subs + s) * SUB + warp * 32 * PER_THREAD + lane;
-#pragma unroll
-    for (int w = 0; w < SORT_WARPS; ++w) before[w][threadIdx.x] = 0;
-    __syncthreads();
     uint2 e[PER_THREAD];
-    uint32_t d[PER_THREAD], rank[PER_THREAD];
+    uint32_t d[PER_THREAD], r[PER_THREAD];
 #pragma unroll
     for (int i = 0; i < PER_THREAD; ++i) {
       const int64_t n = n0 + i * 32;
-      d[i] = RADIX;
-      if (n < p.N) { e[i] = entry(p, n); d[i] = digit(p, e[i].x, p.shift); }
+      e[i] = entry(p, min(n, p.N - 1));
+      d[i] = n < p.N ? digit(p, e[i].x, p.shift) : RADIX;
     }
-    warp_ranks(d, rank, before[warp]);
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < SORT_WARPS; ++w) {
-      const uint32_t c = before[w][threadIdx.x];
-      before[w][threadIdx.x] = base;
-      base += c;
-    }
-    __syncthreads();
+    order.clear();
+    order.rank(d, r);
+    order.place(base);
 #pragma unroll
     for (int i = 0; i < PER_THREAD; ++i)
-      if (d[i] < RADIX) p.out[before[warp][d[i]] + rank[i]] = e[i];
+      if (d[i] < RADIX) p.out[order.at(d[i], r[i])] = e[i];
     __syncthreads();
   }
 }
 
-// All passes of up to SUB ids in the first CTA; the others clear the table.
-__global__ void __launch_bounds__(THREADS) small_sort_kernel(const __grid_constant__ SortParams p) {
-  __shared__ uint32_t before[SORT_WARPS][RADIX], sums[SORT_WARPS];
-  __shared__ uint2 moved[SUB];
+// All passes of up to ONE ids in the first CTA; the others clear the table.
+struct OneShared {
+  Order<ONE_THREADS> order;
+  uint2 moved[ONE];
+};
+__global__ void __launch_bounds__(ONE_THREADS) one_sort_kernel(const __grid_constant__ SortParams p) {
+  extern __shared__ __align__(16) unsigned char dynamic[];
+  OneShared& sh = *reinterpret_cast<OneShared*>(dynamic);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (blockIdx.x > 0) {
-    clear_table(p, blockIdx.x - 1, gridDim.x - 1);
+    clear_table<ONE_THREADS>(p, blockIdx.x - 1, gridDim.x - 1);
     return;
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n0 = warp * 32 * PER_THREAD + lane;
   uint2 e[PER_THREAD];
-  uint32_t d[PER_THREAD], rank[PER_THREAD];
+  uint32_t d[PER_THREAD], r[PER_THREAD];
 #pragma unroll
-  for (int i = 0; i < PER_THREAD; ++i)
-    if (n0 + i * 32 < p.N) e[i] = entry(p, n0 + i * 32);
+  for (int i = 0; i < PER_THREAD; ++i) e[i] = entry(p, min((int64_t)n0 + i * 32, p.N - 1));
   for (int pass = 0; pass < p.passes; ++pass) {
 #pragma unroll
-    for (int w = 0; w < SORT_WARPS; ++w) before[w][threadIdx.x] = 0;
-    __syncthreads();
-#pragma unroll
     for (int i = 0; i < PER_THREAD; ++i) d[i] = n0 + i * 32 < p.N ? digit(p, e[i].x, pass * p.bits) : RADIX;
-    warp_ranks(d, rank, before[warp]);
-    __syncthreads();
+    sh.order.clear();
+    sh.order.rank(d, r);
     uint32_t all = 0;
+    if (threadIdx.x < RADIX) {
 #pragma unroll
-    for (int w = 0; w < SORT_WARPS; ++w) all += before[w][threadIdx.x];
-    uint32_t base = block_scan(all, sums);
-#pragma unroll
-    for (int w = 0; w < SORT_WARPS; ++w) {
-      const uint32_t c = before[w][threadIdx.x];
-      before[w][threadIdx.x] = base;
-      base += c;
+      for (int w = 0; w < ONE_THREADS / 32; ++w) all += sh.order.before[w][threadIdx.x];
     }
+    uint32_t base = sh.order.scan(all);
+    sh.order.place(base);
+#pragma unroll
+    for (int i = 0; i < PER_THREAD; ++i)
+      if (d[i] < RADIX) sh.moved[sh.order.at(d[i], r[i])] = e[i];
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < PER_THREAD; ++i)
-      if (d[i] < RADIX) moved[before[warp][d[i]] + rank[i]] = e[i];
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < PER_THREAD; ++i)
-      if (n0 + i * 32 < p.N) e[i] = moved[n0 + i * 32];
+      if (n0 + i * 32 < p.N) e[i] = sh.moved[n0 + i * 32];
     __syncthreads();
   }
 #pragma unroll
@@ -244,7 +300,10 @@ __global__ void __launch_bounds__(SUM_THREADS) run_sums_kernel(const __grid_cons
   const T* dy = (const T*)p.dy + col;
   uint2 e[AHEAD];
 #pragma unroll
-  for (int j = 0; j < AHEAD; ++j) e[j] = begin + j < end ? p.sorted[begin + j] : make_uint2(p.V, 0);
+  for (int j = 0; j < AHEAD; ++j) {
+    e[j] = p.sorted[min(begin + j, end - 1)];
+    if (begin + j >= end) e[j].x = p.V;
+  }
   uint32_t id = e[0].x;
   if (id == p.V) return;
   bool open = id == before;                // the run in hand began before this window
@@ -269,12 +328,15 @@ __global__ void __launch_bounds__(SUM_THREADS) run_sums_kernel(const __grid_cons
     T single[WIDE ? 1 : AHEAD];
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
-      const T* from = dy + (int64_t)e[j].y * p.dy_stride;         // (an entry behind the last one stands for row 0)
+      const T* from = dy + (int64_t)e[j].y * p.dy_stride;
       if constexpr (WIDE) read8(from, rows[j]); else single[j] = *from;
     }
     uint2 ahead[AHEAD];
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j) ahead[j] = i + AHEAD + j < end ? p.sorted[i + AHEAD + j] : make_uint2(p.V, 0);
+    for (int j = 0; j < AHEAD; ++j) {
+      ahead[j] = p.sorted[min(i + AHEAD + j, end - 1)];
+      if (i + AHEAD + j >= end) ahead[j].x = p.V;
+    }
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
       if (e[j].x != id) {
@@ -300,52 +362,40 @@ __global__ void __launch_bounds__(SUM_THREADS) run_sums_kernel(const __grid_cons
   finish(after == id);
 }
 
-// Four columns a thread, JOIN_SLICES threads for the same columns of a run, each every fourth window of it.
-constexpr int JOIN_COLS = 128, JOIN_SLICES = 4, JOIN_THREADS = JOIN_COLS * JOIN_SLICES;
+// A CTA a window, four columns a thread: the run that begins in the window and goes on, if there is one.
+constexpr int JOIN_THREADS = 128, JOIN_COLS = 4 * JOIN_THREADS;
 
 template <typename T>
 __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constant__ SumParams p) {
-  __shared__ float4 sums[JOIN_SLICES][JOIN_COLS];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int slice = threadIdx.x / JOIN_COLS, lane = threadIdx.x % JOIN_COLS;
-  const int64_t col = ((int64_t)blockIdx.y * JOIN_COLS + lane) * 4;
-  for (int64_t w = blockIdx.x; w + 1 < p.windows; w += gridDim.x) {
-    const int64_t begin = w * p.W, last = begin + p.W - 1;
-    const uint32_t id = p.sorted[last].x;
-    if (id == p.V || p.sorted[last + 1].x != id) continue;                                 // no run goes on behind this window
-    if (p.sorted[begin].x == id && begin > 0 && p.sorted[begin - 1].x == id) continue;     // it began before this window
-    int64_t windows = 1;                                                                    // that it goes through after this one
-    for (;;) {
-      const int64_t first = (w + windows + 1 + threadIdx.x) * p.W;                           // of the window after each of them
-      const int more = __syncthreads_count(first < p.N && p.sorted[first].x == id);         // (the first `more` threads: ids are in order)
-      windows += more;
-      if (more < JOIN_THREADS) break;
-    }
-    float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (col < p.pitch) {
-      if (slice == 0) a = *reinterpret_cast<const float4*>(p.partial + (w * 2 + 1) * p.pitch + col);
-#pragma unroll 8
-      for (int64_t u = w + 1 + slice; u <= w + windows; u += JOIN_SLICES) {
-        const float4 b = *reinterpret_cast<const float4*>(p.partial + u * 2 * p.pitch + col);
-        a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
-      }
-    }
-    sums[slice][lane] = a;
-    __syncthreads();
-    if (slice == 0) {
-#pragma unroll
-      for (int s = 1; s < JOIN_SLICES; ++s) {
-        const float4 b = sums[s][lane];
-        a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
-      }
-      const float f[4] = {a.x, a.y, a.z, a.w};
-      T* to = (T*)p.dw + (int64_t)id * p.D + col;
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (col + c < p.D) to[c] = from_float<T>(f[c] * p.scale);
-    }
-    __syncthreads();
+  const int64_t w = blockIdx.x, begin = w * p.W, last = begin + p.W - 1;                 // (not the last window: there is a next one)
+  const int64_t col = ((int64_t)blockIdx.y * JOIN_THREADS + threadIdx.x) * 4;
+  const uint32_t id = p.sorted[last].x, next = p.sorted[last + 1].x, first = p.sorted[begin].x, before = begin > 0 ? p.sorted[begin - 1].x : p.V;
+  if (id == p.V || next != id) return;                                                   // no run goes on behind this window
+  if (first == id && before == id) return;                                               // it began before this window
+  int64_t windows = 1;                                                                   // that it goes through after this one
+  for (;;) {
+    const int64_t at = (w + windows + 1 + threadIdx.x) * p.W;                            // of the window after each of them
+    const int more = __syncthreads_count(at < p.N && p.sorted[at].x == id);             // (the first `more` threads: ids are in order)
+    windows += more;
+    if (more < JOIN_THREADS) break;
   }
+  if (col >= p.pitch) return;
+  float4 a = *reinterpret_cast<const float4*>(p.partial + (w * 2 + 1) * p.pitch + col);
+  const int64_t end = w + windows;
+  for (int64_t u = w + 1; u <= end; u += 16) {
+    float4 b[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) b[i] = *reinterpret_cast<const float4*>(p.partial + min(u + i, end) * 2 * p.pitch + col);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (u + i <= end) { a.x += b[i].x; a.y += b[i].y; a.z += b[i].z; a.w += b[i].w; }
+  }
+  const float f[4] = {a.x, a.y, a.z, a.w};
+  T* to = (T*)p.dw + (int64_t)id * p.D + col;
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    if (col + c < p.D) to[c] = from_float<T>(f[c] * p.scale);
 }
 
 // How a gradient is cut up, and where its scratch memory lies.
@@ -383,9 +433,17 @@ cudaError_t table_grad(const GradPlan& g, SortParams s, SumParams q, bool wide, 
   constexpr int CLEARING = 592;                    // CTAs
   uint2* buffers[2] = {(uint2*)(space + g.sorted[0]), (uint2*)(space + g.sorted[1])};
   cudaError_t e;
-  if (g.tiles * g.subs == 1) {
+  if (q.N <= ONE) {
+    // (a CTA alone: its passes need no launch, 4 us each, between them)
+    static std::atomic<bool> configured[64];
+    int dev = 0;
+    if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
+      if ((e = cudaFuncSetAttribute(one_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(OneShared))) != cudaSuccess) return e;
+      if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
+    }
     s.out = buffers[0];
-    e = launch_kernel(small_sort_kernel, dim3(1 + CLEARING), THREADS, 0, false, s, stream);
+    e = launch_kernel(one_sort_kernel, dim3(1 + CLEARING / 4), ONE_THREADS, sizeof(OneShared), false, s, stream);
     *n_launched += 1;
     q.sorted = buffers[0];
   } else {
@@ -394,8 +452,8 @@ cudaError_t table_grad(const GradPlan& g, SortParams s, SumParams q, bool wide, 
       s.in = pass == 0 ? nullptr : buffers[(pass - 1) & 1];
       s.out = buffers[pass & 1];
       s.shift = pass * g.bits;
-      e = launch_kernel(digit_counts_kernel, dim3(g.tiles + (pass == 0 ? CLEARING : 0)), THREADS, 0, pass > 0, s, stream);
-      if (e == cudaSuccess) e = launch_kernel(scatter_kernel, dim3(g.tiles), THREADS, 0, true, s, stream);
+      e = launch_kernel(digit_counts_kernel, dim3(g.tiles + (pass == 0 ? CLEARING : 0)), TILE_THREADS, 0, pass > 0, s, stream);
+      if (e == cudaSuccess) e = launch_kernel(scatter_kernel, dim3(g.tiles), TILE_THREADS, 0, true, s, stream);
       *n_launched += 2;
     }
     q.sorted = buffers[(g.passes - 1) & 1];
@@ -410,7 +468,7 @@ cudaError_t table_grad(const GradPlan& g, SortParams s, SumParams q, bool wide, 
            : launch_kernel(run_sums_kernel<T, false>, grid, SUM_THREADS, 0, true, q, stream);
   *n_launched += 1;
   if (e == cudaSuccess && q.windows > 1) {
-    const dim3 joins((unsigned)(q.windows < 592 ? q.windows : 592), (unsigned)((q.D + 4 * JOIN_COLS - 1) / (4 * JOIN_COLS)));
+    const dim3 joins((unsigned)(q.windows - 1), (unsigned)((q.D + JOIN_COLS - 1) / JOIN_COLS));
     e = launch_kernel(join_kernel<T>, joins, JOIN_THREADS, 0, true, q, stream);
     *n_launched += 1;
   }
@@ -422,7 +480,7 @@ cudaError_t lookup(LookupParams p, bool wide, cudaStream_t stream) {
   p.units = wide ? p.D / 8 : p.D;
   p.log_threads = 0;
   while ((1 << p.log_threads) < p.units && p.log_threads < 8) ++p.log_threads;
-  const int rows = THREADS >> p.log_threads;
+  const int rows = (THREADS >> p.log_threads) * ROWS;
   const dim3 grid((unsigned)((p.N + rows - 1) / rows));
   return wide ? launch_kernel(lookup_kernel<T, true>, grid, THREADS, 0, false, p, stream)
               : launch_kernel(lookup_kernel<T, false>, grid, THREADS, 0, false, p, stream);
