@@ -3,16 +3,19 @@
 //   g = R^T dy,  dw = sum over all rows of g n,  dx = r (g w - n mean(g w n))
 // fp32 arithmetic on bf16 or fp32 tensors; bound by HBM: forward one read and one write, backward two reads and one write.
 //
-// A row (token, head) of d <= 256 channels belongs to d / 8 lanes, a power of two of them set aside, eight channels each; such
-// a group of lanes walks over heads of one token - queries, then keys - so that the token's phasors (8 floats a lane) and
-// the weights are read once for all of them.
+// A row (token, head) of d <= 256 channels belongs to d / 8 lanes, a power of two of them set aside, eight channels each: a lane
+// keeps its channels' weights for the whole launch.  A group of lanes takes HEADS heads of a token, which share its phasors, and
+// moves from token to token by adding strides; the arithmetic runs on pairs of floats.  Issue slots and loads in flight both count: with
+// one head at a time, an index worked out for every row and scalar arithmetic 32768 tokens of 8 + 8 heads of 128 took 78 us forward
+// and 112 backward, with two heads, strides and pairs 58 and 103 (cold and dirty caches; 64 registers: 4 CTAs an SM; left to itself
+// the compiler takes 102 and 144, and 75 and 155 us).  fp32 rows need more registers and fewer of them in flight.
 #include "fpb_common.cuh"
 #include "vec_io.cuh"
 
 namespace fpb {
 namespace {
 
-constexpr int THREADS = 256, AHEAD = 4;       // heads a group has in flight
+constexpr int THREADS = 256, ROUNDS = 8;      // tokens in a row, at most
 
 struct QkNormParams {
   SeqView x[2], dy[2], out[2];      // queries, keys: input, upstream gradient (backward), result
@@ -20,124 +23,144 @@ struct QkNormParams {
   const float2* phasors;            // (rows, T, d/2), null: no rotation
   int64_t ph_sb;                    // in float2 units, 0: one table for all batch rows
   float* partial;                   // backward: (CTAs, 2, d) sums of the weights' gradients
-  int64_t tokens;                   // B T
-  int32_t T, H[2], d;
-  int32_t pieces, heads;            // a token's heads are shared out over `pieces` groups, `heads` to each
+  int32_t B, T, H[2], d, rounds;    // rounds: tokens in a row
   float eps, inv_d;
 };
 
+// sum over the row's lanes
 template <int L> __device__ __forceinline__ float group_sum(float v) {
 #pragma unroll
   for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-__device__ __forceinline__ void rotate(float (&v)[8], const float (&c)[4], const float (&s)[4], float sign) {
+// Eight channels as (first of a channel pair) x 4, (second) x 4.
+struct Eight {
+  Pair a[2], b[2];
+};
+__device__ __forceinline__ Eight split(const float (&f)[8]) {
+  return Eight{{pair(f[0], f[2]), pair(f[4], f[6])}, {pair(f[1], f[3]), pair(f[5], f[7])}};
+}
+__device__ __forceinline__ void together(const Eight& v, float (&f)[8]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float a = v[2 * i], b = v[2 * i + 1], t = sign * s[i];
-    v[2 * i] = a * c[i] - b * t;
-    v[2 * i + 1] = a * t + b * c[i];
+  for (int i = 0; i < 2; ++i) {
+    const float2 a = both(v.a[i]), b = both(v.b[i]);
+    f[4 * i] = a.x; f[4 * i + 1] = b.x; f[4 * i + 2] = a.y; f[4 * i + 3] = b.y;
   }
 }
+// each element times one number; elementwise products and sums; the sum of products
+__device__ __forceinline__ Eight times(const Eight& x, float f) {
+  const Pair p = pair(f, f);
+  return Eight{{x.a[0] * p, x.a[1] * p}, {x.b[0] * p, x.b[1] * p}};
+}
+__device__ __forceinline__ Eight times(const Eight& x, const Eight& y) {
+  return Eight{{x.a[0] * y.a[0], x.a[1] * y.a[1]}, {x.b[0] * y.b[0], x.b[1] * y.b[1]}};
+}
+__device__ __forceinline__ Eight plus_times(const Eight& z, const Eight& x, const Eight& y) {
+  return Eight{{fma(x.a[0], y.a[0], z.a[0]), fma(x.a[1], y.a[1], z.a[1])}, {fma(x.b[0], y.b[0], z.b[0]), fma(x.b[1], y.b[1], z.b[1])}};
+}
+__device__ __forceinline__ Eight plus_times(const Eight& z, const Eight& x, float f) {
+  const Pair p = pair(f, f);
+  return Eight{{fma(x.a[0], p, z.a[0]), fma(x.a[1], p, z.a[1])}, {fma(x.b[0], p, z.b[0]), fma(x.b[1], p, z.b[1])}};
+}
+__device__ __forceinline__ float dot(const Eight& x, const Eight& y) {
+  const float2 s = both(fma(x.b[1], y.b[1], fma(x.b[0], y.b[0], fma(x.a[1], y.a[1], x.a[0] * y.a[0]))));
+  return s.x + s.y;
+}
+// rotated by the angles whose (cos, sin) are c, s; `minus`: -s
+__device__ __forceinline__ Eight rotate(const Eight& x, const Pair (&c)[2], const Pair (&s)[2], const Pair (&minus)[2]) {
+  Eight y;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    y.a[i] = fma(x.b[i], minus[i], x.a[i] * c[i]);
+    y.b[i] = fma(x.b[i], c[i], x.a[i] * s[i]);
+  }
+  return y;
+}
 
-template <typename T, int L, bool BWD>
-__global__ void __launch_bounds__(THREADS) qk_norm_kernel(const __grid_constant__ QkNormParams p) {
+template <typename T, int L, int HEADS, bool BWD>
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 2 : 4) qk_norm_kernel(const __grid_constant__ QkNormParams p) {
   constexpr int GROUPS = THREADS / L;
+  const int which = blockIdx.y, H = p.H[which];
+  const SeqView vx = p.x[which], vg = p.dy[which], vo = p.out[which];
   const int group = threadIdx.x / L, lane = threadIdx.x % L, c0 = lane * 8;
   const bool live = c0 < p.d;
-  float w[2][8], dw[2][8];
+  float f[8];
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
+  for (int e = 0; e < 8; ++e) f[e] = live && p.w[which] ? p.w[which][c0 + e] : 1.0f;
+  const Eight w = split(f);
+  const Pair zero = pair(0.0f, 0.0f);
+  Eight dw{{zero, zero}, {zero, zero}};
+
+  // A CTA takes items of (batch row, stretch of tokens, block of heads).
+  const int sets = (H + HEADS - 1) / HEADS, block = min(sets, GROUPS), per = block ? GROUPS / block : 1;      // groups of heads; tokens at a time
+  const int blocks = block ? (sets + block - 1) / block : 0, stretch = per * p.rounds, stretches = (p.T + stretch - 1) / stretch;
+  const int64_t items = (int64_t)p.B * stretches * blocks;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t rest = item / blocks;
+    const int b = (int)(rest / stretches), t0 = (int)(rest % stretches) * stretch + group / block;
+    const int h = ((int)(item % blocks) * block + group % block) * HEADS;
+    const int heads = live && group < per * block ? min(H - h, HEADS) : 0, tokens = (p.T - t0 + per - 1) / per;      // (those left; `rounds` at most)
+    const T* x_at = (const T*)vx.data + b * vx.sb + t0 * vx.st + h * vx.sh + c0;
+    const T* g_at = BWD ? (const T*)vg.data + b * vg.sb + t0 * vg.st + h * vg.sh + c0 : nullptr;
+    T* o_at = (T*)vo.data + b * vo.sb + t0 * vo.st + h * vo.sh + c0;
+    const float4* ph_at = reinterpret_cast<const float4*>(p.phasors + b * p.ph_sb + (int64_t)t0 * (p.d / 2) + lane * 4);
+    const int64_t x_step = per * vx.st, g_step = BWD ? per * vg.st : 0, o_step = per * vo.st;
+    const int ph_step = per * (p.d / 4);
+#pragma unroll 1
+    for (int n = 0; n < p.rounds; ++n) {
+      if (n * per + (int)(rest % stretches) * stretch >= p.T) break;          // (no token left for any group)
+      const bool here = n < tokens;
+      Raw8<T> rx[HEADS], rg[BWD ? HEADS : 1];
+      float4 u = make_float4(1.0f, 0.0f, 1.0f, 0.0f), v = u;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      w[k][e] = live && p.w[k] ? p.w[k][c0 + e] : 1.0f;
-      dw[k][e] = 0.0f;
-    }
-  const int64_t items = p.tokens * p.pieces, stride = (int64_t)gridDim.x * GROUPS;
-  const int64_t rounds = (items + stride - 1) / stride;           // (the same for all groups: the shuffles below need whole warps)
-  const int both = p.H[0] + p.H[1];
-  for (int64_t n = 0; n < rounds; ++n) {
-    const int64_t item = n * stride + (int64_t)blockIdx.x * GROUPS + group;
-    const bool here = item < items;
-    const int64_t token = here ? item / p.pieces : 0;
-    const int first = here ? (int)(item % p.pieces) * p.heads : 0, end = here ? min(first + p.heads, both) : 0;
-    const int64_t b = token / p.T, t = token % p.T;
-    float c[4], s[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { c[i] = 1.0f; s[i] = 0.0f; }
-    if (p.phasors && live && here) {
-      const float4* ph = reinterpret_cast<const float4*>(p.phasors + b * p.ph_sb + t * (p.d / 2) + lane * 4);
-      const float4 u = __ldg(ph), v = __ldg(ph + 1);
-      c[0] = u.x; s[0] = u.y; c[1] = u.z; s[1] = u.w; c[2] = v.x; s[2] = v.y; c[3] = v.z; s[3] = v.w;
-    }
-    for (int h0 = 0; h0 < p.heads; h0 += AHEAD) {
-      Raw8<T> rx[AHEAD], rg[BWD ? AHEAD : 1];
-#pragma unroll
-      for (int j = 0; j < AHEAD; ++j) {
-        const int h = first + h0 + j;
-        if (h < end && live) {
-          const int k = h >= p.H[0];
-          const int64_t hh = k ? h - p.H[0] : h;
-          read8((const T*)p.x[k].data + b * p.x[k].sb + t * p.x[k].st + hh * p.x[k].sh + c0, rx[j]);
-          if constexpr (BWD) read8((const T*)p.dy[k].data + b * p.dy[k].sb + t * p.dy[k].st + hh * p.dy[k].sh + c0, rg[j]);
-        } else {
-          rx[j] = Raw8<T>{};
-          if constexpr (BWD) rg[j] = Raw8<T>{};
+      for (int j = 0; j < HEADS; ++j) {
+        rx[j] = Raw8<T>{};
+        if constexpr (BWD) rg[j] = Raw8<T>{};
+        if (here && j < heads) {
+          read8(x_at + j * vx.sh, rx[j]);
+          if constexpr (BWD) read8(g_at + j * vg.sh, rg[j]);
         }
       }
+      if (p.phasors && here && heads > 0) { u = __ldg(ph_at); v = __ldg(ph_at + 1); }
+      const Pair c[2] = {pair(u.x, u.z), pair(v.x, v.z)}, s[2] = {pair(u.y, u.w), pair(v.y, v.w)}, minus[2] = {pair(-u.y, -u.w), pair(-v.y, -v.w)};
 #pragma unroll
-      for (int j = 0; j < AHEAD; ++j) {
-        const int h = first + h0 + j, k = h >= p.H[0];
-        float x[8], g[8];
-        unpack8(rx[j], x);
-        float sq = 0.0f, dot = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sq += x[e] * x[e];
+      for (int j = 0; j < HEADS; ++j) {
+        unpack8(rx[j], f);
+        const Eight x = split(f);
+        float sq = dot(x, x);
+        Eight y;
         if constexpr (BWD) {
-          unpack8(rg[j], g);
-          rotate(g, c, s, -1.0f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) dot += g[e] * (k ? w[1][e] : w[0][e]) * x[e];
-          dot = group_sum<L>(dot);
-        }
-        const float r = rsqrtf(group_sum<L>(sq) * p.inv_d + p.eps);
-        if (!(h < end && live)) continue;
-        float y[8];
-        if constexpr (BWD) {
-          const float m = dot * r * r * p.inv_d;                  // r mean(g w n), as n = x r
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float gn = g[e] * x[e] * r;
-            if (k) dw[1][e] += gn; else dw[0][e] += gn;
-            y[e] = r * (g[e] * (k ? w[1][e] : w[0][e]) - x[e] * m);
-          }
+          unpack8(rg[j], f);
+          const Eight g = rotate(split(f), c, minus, s), gw = times(g, w);     // back through the rotation, then the weights
+          const float along = group_sum<L>(dot(gw, x));
+          const float r = rsqrtf(group_sum<L>(sq) * p.inv_d + p.eps), m = -along * r * r * p.inv_d;       // -r mean(g w n), as n = x r
+          dw = plus_times(dw, g, times(x, r));
+          y = times(plus_times(gw, x, m), r);
         } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = x[e] * r * (k ? w[1][e] : w[0][e]);
-          rotate(y, c, s, 1.0f);
+          const float r = rsqrtf(group_sum<L>(sq) * p.inv_d + p.eps);
+          y = rotate(times(times(x, r), w), c, s, minus);
         }
-        const int64_t hh = k ? h - p.H[0] : h;
-        store8((T*)p.out[k].data + b * p.out[k].sb + t * p.out[k].st + hh * p.out[k].sh + c0, y);
+        together(y, f);
+        if (here && j < heads) store8(o_at + j * vo.sh, f);
       }
+      x_at += x_step; o_at += o_step; ph_at += ph_step;
+      if constexpr (BWD) g_at += g_step;
     }
   }
   if constexpr (BWD) {
     // the CTA's sums, group after group in a fixed order
     __shared__ float sums[GROUPS][L * 8 + 1];
+    together(dw, f);
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      __syncthreads();
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sums[group][lane + e * L] = dw[k][e];         // (lanes next to one another: no bank twice)
-      __syncthreads();
-      for (int i = threadIdx.x; i < L * 8; i += THREADS) {
-        float a = 0.0f;
+    for (int e = 0; e < 8; ++e) sums[group][lane + e * L] = f[e];               // (lanes next to one another: no bank twice)
+    __syncthreads();
+    for (int i = threadIdx.x; i < L * 8; i += THREADS) {
+      float a = 0.0f;
 #pragma unroll 4
-        for (int q = 0; q < GROUPS; ++q) a += sums[q][i];
-        const int ch = (i % L) * 8 + i / L;
-        if (ch < p.d) p.partial[((int64_t)blockIdx.x * 2 + k) * p.d + ch] = a;
-      }
+      for (int q = 0; q < GROUPS; ++q) a += sums[q][i];
+      const int ch = (i % L) * 8 + i / L;
+      if (ch < p.d) p.partial[((int64_t)blockIdx.x * 2 + which) * p.d + ch] = a;
     }
   }
 }
@@ -165,14 +188,32 @@ __global__ void __launch_bounds__(256) qk_weight_sums_kernel(const __grid_consta
   }
 }
 
-template <typename T, bool BWD>
-cudaError_t launch(const QkNormParams& p, int ctas, cudaStream_t stream) {
-  if (p.d <= 8) return launch_kernel(qk_norm_kernel<T, 1, BWD>, dim3(ctas), THREADS, 0, false, p, stream);
-  if (p.d <= 16) return launch_kernel(qk_norm_kernel<T, 2, BWD>, dim3(ctas), THREADS, 0, false, p, stream);
-  if (p.d <= 32) return launch_kernel(qk_norm_kernel<T, 4, BWD>, dim3(ctas), THREADS, 0, false, p, stream);
-  if (p.d <= 64) return launch_kernel(qk_norm_kernel<T, 8, BWD>, dim3(ctas), THREADS, 0, false, p, stream);
-  if (p.d <= 128) return launch_kernel(qk_norm_kernel<T, 16, BWD>, dim3(ctas), THREADS, 0, false, p, stream);
-  return launch_kernel(qk_norm_kernel<T, 32, BWD>, dim3(ctas), THREADS, 0, false, p, stream);
+template <typename T, int HEADS, bool BWD>
+cudaError_t launch(QkNormParams p, cudaStream_t stream, int* slabs) {
+  int lanes = 1;
+  while (lanes * 8 < p.d) lanes *= 2;
+  const int groups = THREADS / lanes, H = p.H[0] > p.H[1] ? p.H[0] : p.H[1], sets = (H + HEADS - 1) / HEADS, block = sets < groups ? sets : groups;
+  // as many tokens in a row as leave four CTAs an SM over both tensors
+  int64_t items;
+  for (p.rounds = ROUNDS;; p.rounds /= 2) {
+    const int stretch = groups / block * p.rounds;
+    items = (int64_t)p.B * ((p.T + stretch - 1) / stretch) * ((sets + block - 1) / block);
+    if (items >= FPB_QK_NORM_SLABS / 2 || p.rounds == 1) break;
+  }
+  // at most eight CTAs an SM over both tensors; the backward's leave a slab of sums each
+  const dim3 grid((unsigned)(items < FPB_QK_NORM_SLABS ? items : FPB_QK_NORM_SLABS), 2);
+  *slabs = (int)grid.x;
+  switch (lanes) {
+    case 1: return launch_kernel(qk_norm_kernel<T, 1, HEADS, BWD>, grid, THREADS, 0, false, p, stream);
+    case 2: return launch_kernel(qk_norm_kernel<T, 2, HEADS, BWD>, grid, THREADS, 0, false, p, stream);
+    case 4: return launch_kernel(qk_norm_kernel<T, 4, HEADS, BWD>, grid, THREADS, 0, false, p, stream);
+    case 8: return launch_kernel(qk_norm_kernel<T, 8, HEADS, BWD>, grid, THREADS, 0, false, p, stream);
+    case 16: return launch_kernel(qk_norm_kernel<T, 16, HEADS, BWD>, grid, THREADS, 0, false, p, stream);
+    default: return launch_kernel(qk_norm_kernel<T, 32, HEADS, BWD>, grid, THREADS, 0, false, p, stream);
+  }
+}
+template <typename T, bool BWD> cudaError_t launch(const QkNormParams& p, cudaStream_t stream, int* slabs) {
+  return p.H[0] > 1 || p.H[1] > 1 ? launch<T, 2, BWD>(p, stream, slabs) : launch<T, 1, BWD>(p, stream, slabs);
 }
 
 }  // namespace
@@ -183,23 +224,15 @@ int launch_qk_norm(int dtype, bool backward, int B, int T, int Hq, int Hk, int d
   QkNormParams p{};
   for (int k = 0; k < 2; ++k) { p.x[k] = x[k]; p.out[k] = out[k]; p.w[k] = w[k]; if (backward) p.dy[k] = dy[k]; }
   p.phasors = (const float2*)phasors; p.ph_sb = phasor_stride_b; p.partial = partial;
-  p.tokens = (int64_t)B * T; p.T = T; p.H[0] = Hq; p.H[1] = Hk; p.d = d; p.eps = eps; p.inv_d = 1.0f / (float)d;
-  int lanes = 1;
-  while (lanes * 8 < d) lanes *= 2;
-  const int groups = THREADS / lanes, most = FPB_QK_NORM_SLABS;
-  // all heads of a token to one group where that leaves a group for every slot of the GPU, else four heads (one round of
-  // loads), so that a few tokens spread over the SMs
-  p.heads = p.tokens >= (int64_t)most * groups ? Hq + Hk : AHEAD;
-  p.pieces = (Hq + Hk + p.heads - 1) / p.heads;
-  const int64_t ctas = (p.tokens * p.pieces + groups - 1) / groups;
-  const int grid = (int)(ctas < most ? ctas : most);
+  p.B = B; p.T = T; p.H[0] = Hq; p.H[1] = Hk; p.d = d; p.eps = eps; p.inv_d = 1.0f / (float)d;
   cudaError_t e;
+  int slabs = 0;
   if (!backward) {
-    e = dtype == FPB_BF16 ? launch<__nv_bfloat16, false>(p, grid, stream) : launch<float, false>(p, grid, stream);
+    e = dtype == FPB_BF16 ? launch<__nv_bfloat16, false>(p, stream, &slabs) : launch<float, false>(p, stream, &slabs);
   } else {
-    e = dtype == FPB_BF16 ? launch<__nv_bfloat16, true>(p, grid, stream) : launch<float, true>(p, grid, stream);
+    e = dtype == FPB_BF16 ? launch<__nv_bfloat16, true>(p, stream, &slabs) : launch<float, true>(p, stream, &slabs);
     if (e == cudaSuccess && (dw[0] || dw[1])) {
-      const QkSumParams s{partial, {dw[0], dw[1]}, d, grid};
+      const QkSumParams s{partial, {dw[0], dw[1]}, d, slabs};
       e = launch_kernel(qk_weight_sums_kernel, dim3((2 * d + 31) / 32), 256, 0, false, s, stream);
     }
   }

@@ -15,6 +15,7 @@
 namespace fpb {
 namespace {
 
+// (the row's arithmetic is issue-bound beside the memory it reads: pairs of floats, vec_io.cuh)
 constexpr float LEAST = -1e4f;
 constexpr unsigned ALL = 0xffffffffu;
 
@@ -32,36 +33,6 @@ __device__ __forceinline__ float exp2_of(float x) {
   return r;
 }
 constexpr float LOG2E = 1.44269504088896f, LN2 = 0.693147180559945f;
-
-// Two floats to an instruction: the row's arithmetic is issue-bound beside the memory it reads.
-struct Pair {
-  uint64_t v;
-};
-__device__ __forceinline__ Pair pair(float a, float b) {
-  Pair r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 both(Pair a) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
-  return r;
-}
-__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
-  Pair r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
-  Pair r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
-  Pair r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
 
 // ---- a row as vectors -----------------------------------------------------------------------------------------------
 // A row starts at any element: it is so many single elements up to a 16-byte boundary, whole vectors, and a rest.
