@@ -143,11 +143,20 @@ template <typename T, int N> __device__ __noinline__ float2 careful_sums(const V
 }
 
 // The largest of a thread's vectors, of which the first `count` are of the row.
-template <typename T, int N> __device__ __forceinline__ float largest_of(const Vectors<N>& from, int count) {
-  float most = largest<T>(from.r[0]);
+template <typename T, bool FULL, int N> __device__ __forceinline__ float largest_of(const Vectors<N>& from, int count) {
+  float most;
+  if constexpr (sizeof(T) == 2) {
+    auto h = [&](int j, int i) { const uint32_t w = word(from.r[j], i); return *reinterpret_cast<const __nv_bfloat162*>(&w); };
+    __nv_bfloat162 m = h(0, 0);
 #pragma unroll
-  for (int j = 1; j < N; ++j) most = max_nan(most, largest<T>(from.r[j]));
-  if (count < N && !(most > FILL)) {                 // (what stands for those behind the row is more than a mask's value)
+    for (int i = 1; i < 4 * N; ++i) m = __hmax2_nan(m, h(i / 4, i % 4));
+    most = max_nan(__low2float(m), __high2float(m));
+  } else {
+    most = largest<T>(from.r[0]);
+#pragma unroll
+    for (int j = 1; j < N; ++j) most = max_nan(most, largest<T>(from.r[j]));
+  }
+  if (!FULL && count < N && !(most > FILL)) {        // (what stands for those behind the row is more than a mask's value)
     most = -INFINITY;
 #pragma unroll
     for (int j = 0; j < N; ++j)
@@ -157,7 +166,7 @@ template <typename T, int N> __device__ __forceinline__ float largest_of(const V
 }
 
 // N vectors of a thread, of which the first `count` are of the row and the first `slots` are of some thread's; most: their largest
-template <typename T, int N> __device__ __forceinline__ void add(Stats& a, const Vectors<N>& from, int count, int slots, float most) {
+template <typename T, bool FULL, int N> __device__ __forceinline__ void add(Stats& a, const Vectors<N>& from, int count, int slots, float most) {
   const float m = max_nan(a.m, most);
   if (m == -INFINITY) return;
   if (m != a.m) move_to(a, m);
@@ -166,7 +175,7 @@ template <typename T, int N> __device__ __forceinline__ void add(Stats& a, const
   Pair s = pair(0.0f, 0.0f), t = s;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    if (j >= slots) break;
+    if (!FULL && j >= slots) break;
 #pragma unroll
     for (int i = 0; i < Row<T>::E / 2; ++i) {
       const Pair y = fma(elements<T>(from.r[j], i), log2e, minus);
@@ -328,12 +337,16 @@ template <typename T, int NT> __device__ __noinline__ void exact_candidates(cons
   __syncthreads();
 }
 
-// The largest maxima of the parts that a tile is cut into, sorted, one a lane of every warp: 32 parts, or 64 where more than FEW
-// alternatives are wanted.  `most`: a thread's maximum.  One barrier.
-template <int NT> __device__ __forceinline__ uint32_t part_maxima(float most, bool few, uint32_t (&group)[64]) {
+// The maxima of the parts that the tiles seen are cut into, 32 or, where more than FEW alternatives are wanted, 64; one or two a lane
+// of every warp.  A part is the same threads' share of every tile.
+struct Parts {
+  uint32_t a = 0, b = 0;
+};
+// `most`: a thread's maximum of this tile.  One barrier, but with a single warp.
+template <int NT> __device__ __forceinline__ void add_maxima(Parts& parts, float most, bool few, uint32_t (&group)[64]) {
   const int lane = threadIdx.x & 31;
   uint32_t g = order_of(most);
-  if (NT == 32) return sort_warp(g);
+  if (NT == 32) { parts.a = max(parts.a, g); return; }
 #pragma unroll
   for (int o = 1; o < NT / 64; o *= 2) g = max(g, __shfl_xor_sync(ALL, g, o));
   if (few) {
@@ -343,8 +356,15 @@ template <int NT> __device__ __forceinline__ uint32_t part_maxima(float most, bo
     group[threadIdx.x / (NT / 64 ? NT / 64 : 1)] = g;
   }
   __syncthreads();
-  const uint32_t sorted = sort_warp(group[lane]);
-  return few ? sorted : merge_sorted(sorted, sort_warp(group[32 + lane]));
+  parts.a = max(parts.a, group[lane]);
+  if (!few) parts.b = max(parts.b, group[32 + lane]);
+}
+// the top-th largest of them
+__device__ __forceinline__ uint32_t kth(const Parts& parts, int top) {
+  if (top == 1) return __reduce_max_sync(ALL, parts.a);
+  uint32_t sorted = sort_warp(parts.a);
+  if (top > FEW) sorted = merge_sorted(sorted, sort_warp(parts.b));
+  return __shfl_sync(ALL, sorted, top - 1);
 }
 
 // The elements of a thread's vectors that reach the bound join the candidates, as far as there is room.  STRICT: those at a bound
@@ -375,10 +395,11 @@ template <typename T, int NT> __device__ __noinline__ void careful_candidates(co
   for (int first = begin, parity = 0; first < end; first += U * NT, parity ^= 1) {
     Tile tile;
     row.template read<NT>(tile, first, end);
-    const float most = largest_of<T>(tile, (end - first - (int)threadIdx.x + NT - 1) / NT);
-    const uint32_t sorted = part_maxima<NT>(most, top <= FEW, sh.group[parity]);
+    const float most = largest_of<T, false>(tile, (end - first - (int)threadIdx.x + NT - 1) / NT);
+    Parts parts;
+    add_maxima<NT>(parts, most, top <= FEW, sh.group[parity]);
     if (NT == 32) __syncthreads();
-    least = max(least, __shfl_sync(ALL, sorted, top - 1));
+    least = max(least, kth(parts, top));
     const float bound = value_of(least);
     if (!(most < bound)) push<T, NT, false>(row, tile, first, end, bound, sh);
     __syncthreads();
@@ -394,6 +415,18 @@ template <typename T, int NT> __device__ __noinline__ void careful_candidates(co
     kept = sh.found;
     __syncthreads();
   }
+}
+
+// now, wherever the value is used
+__device__ __forceinline__ float load_now(const float* p) {
+  float v;
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ float load_now(const __nv_bfloat16* p) {
+  uint16_t v;
+  asm volatile("ld.global.u16 %0, [%1];" : "=h"(v) : "l"(p));
+  return __uint_as_float((uint32_t)v << 16);
 }
 
 // One pass over the row, the next vectors on their way while these are added.  Alternatives: a thread whose N vectors reach the
@@ -421,36 +454,54 @@ __global__ void __launch_bounds__(NT, 1024 / NT) scores_kernel(const __grid_cons
   // `top` parts of the tiles seen reach the top-th largest of the parts' maxima: so many elements do, and of any order of the
   // elements not many more are to be expected (of one tile 32 ln(32 / (32 - top))).  The bound is taken again when as many
   // tiles have passed as before: it lets about as many through from one time to the next.
-  uint32_t parts = 0;                                // the largest maxima, one a lane
+  Parts parts;
   float bound = -INFINITY;
   if constexpr (TOP) {
     if (threadIdx.x == 0) sh.records = sh.found = 0;
     if (NT == 32) __syncthreads();
   }
 
-  Vectors<N> now, next;
-  row.template read<NT>(now, begin, end);
-  for (int first = begin, i = 0; first < end; first += N * NT, ++i) {
-    row.template read<NT>(next, first + N * NT, end);
-    const int count = (end - first - (int)threadIdx.x + NT - 1) / NT;
-    const float most = largest_of<T>(now, count);
-    add<T, N>(a, now, count, (end - first + NT - 1) / NT, most);
+  auto take = [&](auto full, const Vectors<N>& tile, int first, int i) {
+    constexpr bool FULL = decltype(full)::value;
+    const int count = FULL ? N : (end - first - (int)threadIdx.x + NT - 1) / NT;
+    const float most = largest_of<T, FULL>(tile, count);
+    add<T, FULL>(a, tile, count, FULL ? N : (end - first + NT - 1) / NT, most);
     if constexpr (TOP) {
       if ((i & (i + 1)) == 0) {
-        const uint32_t sorted = part_maxima<NT>(most, p.top <= FEW, sh.group[__popc(i) & 1]);
-        parts = i == 0 ? sorted : merge_sorted(parts, sorted);
-        bound = value_of(__shfl_sync(ALL, parts, p.top - 1));
+        add_maxima<NT>(parts, most, p.top <= FEW, sh.group[__popc(i) & 1]);
+        bound = value_of(kth(parts, p.top));
       }
       // (a bound as low as a mask's value: only what is above it, the rest of the choice is made below)
       if (bound < SMALLEST ? !(most <= bound) : !(most < bound)) {
         if (end - begin <= N * NT) {                 // (all there is: nothing to wait for)
-          push<T, NT, true>(row, now, first, end, bound, sh);
+          push<T, NT, true>(row, tile, first, end, bound, sh);
         } else {
           const int at = atomicAdd(&sh.records, 1);
           if (at < RECORDS) sh.record[at] = make_uint2(order_of(most), (uint32_t)(first + threadIdx.x));
         }
       }
     }
+  };
+  const std::true_type whole{};
+  const std::false_type part{};
+  Vectors<N> now, next;
+  int first = begin, i = 0;
+  row.template read<NT>(now, first, end);
+  float given = 0.0f;                                // the token's logit, behind the first vectors instead of at the end
+  bool inside = false;
+  if (threadIdx.x == 0) {
+    const int64_t t = p.tokens[n];
+    inside = t >= 0 && t < p.V;
+    given = load_now(row.z + (inside ? t : 0));
+  }
+  for (; first + N * NT <= end; first += N * NT, ++i) {
+    row.template read<NT>(next, first + N * NT, end);
+    take(whole, now, first, i);
+    now = next;
+  }
+  for (; first < end; first += N * NT, ++i) {
+    row.template read<NT>(next, first + N * NT, end);
+    take(part, now, first, i);
     now = next;
   }
 
@@ -474,7 +525,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) scores_kernel(const __grid_cons
     int found = sh.found;
     if (masked && records <= RECORDS && found < p.top) {
       // A row of masked elements but for a few: of the first elements at the bound there are enough, as a rule.
-      __syncthreads();
+      __syncthreads();                               // (all have read `found`)
       const int there = (end - begin) * E;
       for (int i = threadIdx.x; i < 4 * p.top && i < there; i += NT) {
         const float z = to_float(row.z[row.index(begin, i)]);
@@ -485,8 +536,11 @@ __global__ void __launch_bounds__(NT, 1024 / NT) scores_kernel(const __grid_cons
       if (found < p.top && there > 4 * p.top) found = CANDIDATES + 1;
     }
     if (records > RECORDS || found > CANDIDATES) careful_candidates<T, NT>(row, begin, end, p.top, sh);
-    if (has_edge && !(edge < bound)) sh.candidate[atomicAdd(&sh.found, 1)] = rank_key(edge, row.edge(threadIdx.x));
-    __syncthreads();
+    if (share == 0 && row.edges()) {
+      __syncthreads();                               // (all have read `found`)
+      if (has_edge && !(edge < bound)) sh.candidate[atomicAdd(&sh.found, 1)] = rank_key(edge, row.edge(threadIdx.x));
+      __syncthreads();
+    }
     kept = sh.found;
   }
 
@@ -517,8 +571,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) scores_kernel(const __grid_cons
   const bool empty = a.m == -INFINITY;
   const float ls = log_sum(a);
   if (threadIdx.x == 0) {
-    const int64_t t = p.tokens[n];
-    p.logprob[n] = t >= 0 && t < p.V ? (empty ? -INFINITY : (to_float(row.z[t]) - a.m) - ls) : 0.0f;
+    p.logprob[n] = inside ? (empty ? -INFINITY : (given - a.m) - ls) : 0.0f;
     p.entropy[n] = entropy_of(a);
     p.stats[2 * n] = a.m;
     p.stats[2 * n + 1] = ls;
