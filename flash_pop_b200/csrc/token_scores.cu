@@ -57,6 +57,7 @@ template <typename T> struct Row {
   // a thread's vectors tile + its number, and every NT-th after it; those from `end` on are filled with a value that no sum feels
   template <int NT, int N> __device__ __forceinline__ void read(Vectors<N>& to, int tile, int end) const {
     const uint4* from = base() + tile + threadIdx.x;
+    if (NT == 32 && tile >= end) return;             // (never looked at; for longer rows the check costs more than it saves)
     if (tile + N * NT <= end) {
 #pragma unroll
       for (int j = 0; j < N; ++j) to.r[j] = from[j * NT];
@@ -117,13 +118,12 @@ template <int LANES> __device__ __forceinline__ void join(Stats& a) {
     a.t += __shfl_xor_sync(ALL, a.t, o);
   }
 }
-__device__ __forceinline__ float log_sum(const Stats& a) {       // log of the sum of exp(z - m)
-  if (a.m == -INFINITY) return 0.0f;
-  if (a.m == INFINITY) return NAN;
-  return logf(a.s) - (ordinary(a.m) ? LN2 * fmaf(a.m, LOG2E, -origin(a.m)) : 0.0f);
-}
-__device__ __forceinline__ float entropy_of(const Stats& a) {
-  return a.m == -INFINITY ? 0.0f : a.m == INFINITY ? NAN : logf(a.s) - LN2 * (a.t / a.s);
+// log of the sum of exp(z - m), and the entropy
+__device__ __forceinline__ float2 results(const Stats& a) {
+  if (a.m == -INFINITY) return make_float2(0.0f, 0.0f);
+  if (a.m == INFINITY) return make_float2(NAN, NAN);
+  const float log_s = logf(a.s);
+  return make_float2(log_s - (ordinary(a.m) ? LN2 * fmaf(a.m, LOG2E, -origin(a.m)) : 0.0f), log_s - LN2 * __fdividef(a.t, a.s));
 }
 
 // The sums of `count` vectors where the ordinary way meets 0 * -inf (masked elements) or does not apply.
@@ -367,19 +367,20 @@ __device__ __forceinline__ uint32_t kth(const Parts& parts, int top) {
   return __shfl_sync(ALL, sorted, top - 1);
 }
 
-// The elements of a thread's vectors that reach the bound join the candidates, as far as there is room.  STRICT: those at a bound
-// as low as a mask's value do not.
-template <typename T, int NT, bool STRICT, int N> __device__ __forceinline__ void push(const Row<T>& row, const Vectors<N>& from, int first, int end, float bound,
+// The elements of a thread's vectors that reach the bound join the candidates, as far as there is room.
+template <typename T, int NT, int N> __device__ __forceinline__ void push(const Row<T>& row, const Vectors<N>& from, int first, int end, float bound,
                                                                          Shared<NT / 32>& sh) {
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const int v = first + j * NT + threadIdx.x;
-    if (v >= end || largest<T>(from.r[j]) < bound) continue;
+    unsigned reach = 0;
 #pragma unroll
-    for (int e = 0; e < Row<T>::E; ++e) {
-      const float z = element<T>(from.r[j], e);
-      if (z < bound || (STRICT && bound < SMALLEST && z == bound)) continue;
-      const int at = atomicAdd(&sh.found, 1);
+    for (int e = 0; e < Row<T>::E; ++e) reach |= element<T>(from.r[j], e) < bound ? 0u : 1u << e;
+    if (v >= end) reach = 0;
+    for (; reach; reach &= reach - 1) {
+      const int e = __ffs(reach) - 1, at = atomicAdd(&sh.found, 1);
+      const uint32_t w = word(from.r[j], sizeof(T) == 2 ? e / 2 : e);
+      const float z = __uint_as_float(sizeof(T) == 2 ? (e & 1 ? w & 0xffff0000u : w << 16) : w);
       if (at < CANDIDATES) sh.candidate[at] = rank_key(z, row.index(v, e));
     }
   }
@@ -401,7 +402,7 @@ template <typename T, int NT> __device__ __noinline__ void careful_candidates(co
     if (NT == 32) __syncthreads();
     least = max(least, kth(parts, top));
     const float bound = value_of(least);
-    if (!(most < bound)) push<T, NT, false>(row, tile, first, end, bound, sh);
+    if (!(most < bound)) push<T, NT>(row, tile, first, end, bound, sh);
     __syncthreads();
     if (sh.found > CANDIDATES) {
       // no room: the `top` best that earlier tiles left, and this tile's
@@ -455,7 +456,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) scores_kernel(const __grid_cons
   // elements not many more are to be expected (of one tile 32 ln(32 / (32 - top))).  The bound is taken again when as many
   // tiles have passed as before: it lets about as many through from one time to the next.
   Parts parts;
-  float bound = -INFINITY;
+  uint32_t least = order_of(-INFINITY);              // the bound's order; `bound`: the smallest value that counts
+  bool masked = true;
+  float bound = value_of(least + masked);
   if constexpr (TOP) {
     if (threadIdx.x == 0) sh.records = sh.found = 0;
     if (NT == 32) __syncthreads();
@@ -469,12 +472,14 @@ __global__ void __launch_bounds__(NT, 1024 / NT) scores_kernel(const __grid_cons
     if constexpr (TOP) {
       if ((i & (i + 1)) == 0) {
         add_maxima<NT>(parts, most, p.top <= FEW, sh.group[__popc(i) & 1]);
-        bound = value_of(kth(parts, p.top));
+        least = kth(parts, p.top);
+        // (a bound as low as a mask's value: only what is above it, the rest of the choice is made below)
+        masked = value_of(least) < SMALLEST;
+        bound = value_of(least + masked);
       }
-      // (a bound as low as a mask's value: only what is above it, the rest of the choice is made below)
-      if (bound < SMALLEST ? !(most <= bound) : !(most < bound)) {
-        if (end - begin <= N * NT) {                 // (all there is: nothing to wait for)
-          push<T, NT, true>(row, tile, first, end, bound, sh);
+      if (!(most < bound)) {
+        if (NT == 32 && end - begin <= N * NT) {     // (all there is: nothing to wait for; with more threads its code costs the rest)
+          push<T, NT>(row, tile, first, end, bound, sh);
         } else {
           const int at = atomicAdd(&sh.records, 1);
           if (at < RECORDS) sh.record[at] = make_uint2(order_of(most), (uint32_t)(first + threadIdx.x));
@@ -508,15 +513,13 @@ __global__ void __launch_bounds__(NT, 1024 / NT) scores_kernel(const __grid_cons
   if constexpr (TOP) {
     __syncthreads();
     const int records = sh.records;
-    const bool masked = bound < SMALLEST;
     if (records <= RECORDS) {
-      const uint32_t least = bound == -INFINITY ? 0 : order_of(bound);
       for (int q = warp; q < records; q += WARPS) {
         const uint2 at = sh.record[q];
         const int v = (int)at.y + lane / E * NT;
         if (at.x < least || lane >= N * E || v >= end) continue;
         const float z = to_float(row.z[row.index(v, lane % E)]);
-        if (z < bound || (masked && z == bound)) continue;
+        if (z < bound) continue;
         const int to = atomicAdd(&sh.found, 1);
         if (to < CANDIDATES) sh.candidate[to] = rank_key(z, row.index(v, lane % E));
       }
@@ -529,7 +532,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) scores_kernel(const __grid_cons
       const int there = (end - begin) * E;
       for (int i = threadIdx.x; i < 4 * p.top && i < there; i += NT) {
         const float z = to_float(row.z[row.index(begin, i)]);
-        if (z == bound) sh.candidate[atomicAdd(&sh.found, 1)] = rank_key(z, row.index(begin, i));
+        if (order_of(z) == least) sh.candidate[atomicAdd(&sh.found, 1)] = rank_key(z, row.index(begin, i));
       }
       __syncthreads();
       found = sh.found;
@@ -538,7 +541,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) scores_kernel(const __grid_cons
     if (records > RECORDS || found > CANDIDATES) careful_candidates<T, NT>(row, begin, end, p.top, sh);
     if (share == 0 && row.edges()) {
       __syncthreads();                               // (all have read `found`)
-      if (has_edge && !(edge < bound)) sh.candidate[atomicAdd(&sh.found, 1)] = rank_key(edge, row.edge(threadIdx.x));
+      if (has_edge && order_of(edge) >= least) sh.candidate[atomicAdd(&sh.found, 1)] = rank_key(edge, row.edge(threadIdx.x));
       __syncthreads();
     }
     kept = sh.found;
@@ -569,10 +572,11 @@ __global__ void __launch_bounds__(NT, 1024 / NT) scores_kernel(const __grid_cons
     join<32>(a);
   }
   const bool empty = a.m == -INFINITY;
-  const float ls = log_sum(a);
+  const float2 sums_of = results(a);
+  const float ls = sums_of.x;
   if (threadIdx.x == 0) {
     p.logprob[n] = inside ? (empty ? -INFINITY : (given - a.m) - ls) : 0.0f;
-    p.entropy[n] = entropy_of(a);
+    p.entropy[n] = sums_of.y;
     p.stats[2 * n] = a.m;
     p.stats[2 * n + 1] = ls;
   }
