@@ -36,46 +36,63 @@ __device__ __forceinline__ uint4 philox(uint64_t counter, uint32_t k0, uint32_t 
   return make_uint4(c0, c1, c2, c3);
 }
 
-// One group of eight elements a thread.  WIDE: 16-byte accesses (pointers 16-byte aligned).
+// GROUPS groups of eight elements a thread, a CTA's width apart.  WIDE: 16-byte accesses (pointers 16-byte aligned).
+// Four groups share the rounds' keys and have their loads in flight together: 33.5M bf16 elements 37 -> 31 us (66 of 134 MB are
+// still in the caches when it ends), with a residual 39; the integer products are what it issues most.
+constexpr int GROUPS = 4;
 template <typename T, bool WIDE, bool RES>
 __global__ void __launch_bounds__(THREADS) dropout_kernel(const __grid_constant__ DropoutParams p) {
-  const uint64_t seed = (uint64_t)*p.seed;
-  const int64_t group = (int64_t)blockIdx.x * THREADS + threadIdx.x, i0 = group * 8;
-  if (i0 >= p.n) return;
-  const T *x = (const T*)p.x + i0, *r = (const T*)p.residual + i0;
-  T* y = (T*)p.y + i0;
-  const bool whole = i0 + 8 <= p.n;
-  float v[8], s[8];
-  if (WIDE && whole) {
-    load8(x, v);
-    if constexpr (RES) load8(r, s);
-  } else {
+  const int64_t first = (int64_t)blockIdx.x * (THREADS * GROUPS) + threadIdx.x;
+  const T *x = (const T*)p.x, *r = (const T*)p.residual;
+  T* y = (T*)p.y;
+  Raw8<T> rx[GROUPS], rr[RES ? GROUPS : 1];
+  if constexpr (WIDE) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      v[e] = i0 + e < p.n ? to_float(x[e]) : 0.0f;
-      if constexpr (RES) s[e] = i0 + e < p.n ? to_float(r[e]) : 0.0f;
+    for (int j = 0; j < GROUPS; ++j) {
+      const int64_t i0 = (first + j * THREADS) * 8;
+      if (i0 + 8 > p.n) continue;
+      read8(x + i0, rx[j]);
+      if constexpr (RES) read8(r + i0, rr[j]);
     }
   }
-  const uint4 w = philox((uint64_t)group, (uint32_t)seed, (uint32_t)(seed >> 32));
-  const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+  const uint64_t seed = (uint64_t)*p.seed;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const uint32_t half = e & 1 ? words[e >> 1] >> 16 : words[e >> 1] & 0xffffu;
-    v[e] = half >= p.threshold ? v[e] * p.factor : 0.0f;          // (selected, not multiplied: what goes leaves no NaN behind)
-    if constexpr (RES) v[e] += s[e];
-  }
-  if (WIDE && whole) {
-    store8(y, v);
-  } else {
+  for (int j = 0; j < GROUPS; ++j) {
+    const int64_t group = first + j * THREADS, i0 = group * 8;
+    if (i0 >= p.n) return;
+    const bool whole = WIDE && i0 + 8 <= p.n;
+    float v[8], s[8];
+    if (whole) {
+      unpack8(rx[j], v);
+      if constexpr (RES) unpack8(rr[j], s);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (i0 + e < p.n) y[e] = from_float<T>(v[e]);
+      for (int e = 0; e < 8; ++e) {
+        v[e] = i0 + e < p.n ? to_float(x[i0 + e]) : 0.0f;
+        if constexpr (RES) s[e] = i0 + e < p.n ? to_float(r[i0 + e]) : 0.0f;
+      }
+    }
+    const uint4 w = philox((uint64_t)group, (uint32_t)seed, (uint32_t)(seed >> 32));
+    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t half = e & 1 ? words[e >> 1] >> 16 : words[e >> 1] & 0xffffu;
+      v[e] = half >= p.threshold ? v[e] * p.factor : 0.0f;        // (selected, not multiplied: what goes leaves no NaN behind)
+      if constexpr (RES) v[e] += s[e];
+    }
+    if (whole) {
+      store8(y + i0, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (i0 + e < p.n) y[i0 + e] = from_float<T>(v[e]);
+    }
   }
 }
 
 template <typename T>
 cudaError_t launch(const DropoutParams& p, bool wide, cudaStream_t stream) {
-  const dim3 grid((unsigned)((p.n + 8 * THREADS - 1) / (8 * THREADS)));
+  const dim3 grid((unsigned)((p.n + 8 * THREADS * GROUPS - 1) / (8 * THREADS * GROUPS)));
   if (wide)
     return p.residual ? launch_kernel(dropout_kernel<T, true, true>, grid, THREADS, 0, false, p, stream)
                       : launch_kernel(dropout_kernel<T, true, false>, grid, THREADS, 0, false, p, stream);
