@@ -874,7 +874,7 @@ const char* fpb_strerror(int status) {
   }
 }
 
-int fpb_version(void) { return 200; }
+int fpb_version(void) { return 300; }
 
 int64_t fpb_workspace_bytes(const fpb_dims* dims) {
   // what lets the emptiest pass of this shape (one CTA per batch row and head) split as far as it would

@@ -596,6 +596,9 @@ template <typename T, int NT> cudaError_t scores(const ScoreParams& p, cudaStrea
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = (unsigned)p.split; attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr; cfg.numAttrs = p.split > 1 ? 1 : 0;
+#ifdef FPB_DIAGNOSTICS
+  if (launch_refused()) cfg.blockDim = dim3(0);
+#endif
   return p.top ? cudaLaunchKernelEx(&cfg, scores_kernel<T, NT, true>, p) : cudaLaunchKernelEx(&cfg, scores_kernel<T, NT, false>, p);
 }
 

@@ -280,7 +280,7 @@ class RetNetDecoderLayer(nn.Module):
     def _adds_dropout(self) -> bool:
         """Whether what a branch drops is added to the residual in the same pass."""
         return (self.norm_first and type(self.dropout) is CounterDropout and self.dropout.active()
-                and type(self)._residual_blocks is RetNetDecoderLayer._residual_blocks)
+                and type(self)._residual_blocks is RetNetDecoderLayer._residual_blocks and "_residual_blocks" not in self.__dict__)
 
     def _residual_blocks(self, x: Tensor, retention_fn: Callable[[Tensor], Tuple[Tensor, Tensor]], fp32_norm: bool, drop: bool = False):
         """x + retention, x + feed-forward, with the norm before (pre-norm) or after each branch.  `drop`: the retention still has
@@ -291,7 +291,8 @@ class RetNetDecoderLayer(nn.Module):
             y, state = retention_fn(norm(self.norm1, x))
             x = self.dropout(y, x) if drop else x + y
             h = norm(self.norm2, x)
-            if self._adds_dropout() and type(self)._feedforward_block is RetNetDecoderLayer._feedforward_block:
+            if (self._adds_dropout() and type(self)._feedforward_block is RetNetDecoderLayer._feedforward_block
+                    and "_feedforward_block" not in self.__dict__):
                 x = self.dropout(self.linear2(self.dropout(self.activation(self.linear1(h)))), x)
             else:
                 x = x + self._feedforward_block(h)

@@ -50,6 +50,8 @@ class RetNetLM(nn.Module):
         """What the model says of `tokens` (B, T): for each of positions 1 to T-1 the log probability of the token that stands there,
         the entropy of the distribution it came from and, with `top`, the most likely tokens with their log probabilities; all
         (B, T-1[, top]), differentiable."""
+        if tokens.size(1) < 2:                     # nothing before the first token to say anything of it
+            return token_scores(self.head.weight.new_empty((tokens.size(0), 0, self.head.out_features)), tokens[:, 1:], top)
         logits, _ = self(tokens[:, :-1])
         return token_scores(logits, tokens[:, 1:], top)
 

@@ -380,7 +380,8 @@ int fpb_embedding_bwd(int64_t N, int64_t V, int32_t D, int32_t dtype, const int6
  * stats: (rows, 2) floats that the backward reads.  A row of -inf only gives log probabilities of -inf and entropy 0; NaN or +inf
  * in a row make its numbers NaN.
  * The backward writes the gradient of the logits, in their type, from those of the three results (each may be NULL): every
- * element of the row, rows `d_stride` apart, zero for a row of -inf only.  `entropy`, `stats` and `top_tokens` are the forward's.
+ * element of the row, rows `d_stride` apart, zero for a row of -inf only.  `entropy`, `stats` and `top_tokens` are the forward's; d_logits
+ * may not overlap the logits.
  */
 #define FPB_MAX_TOP 32
 int fpb_token_scores_fwd(int64_t rows, int32_t V, int32_t dtype, int32_t top, const void* logits, int64_t row_stride, const int64_t* tokens,

@@ -63,6 +63,12 @@ def test_repeated_missing_and_foreign_ids(D):
     _check(mixed, V, D, F32, padding=-1)
 
 
+def test_more_ids_than_the_sort_has_tiles_for():
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for N, V in ((1_100_000, 3000), (2_200_003, 40), (1_048_577, 200_000)):
+        _check(torch.randint(-1, V, (N,), generator=g, device="cuda"), V, 8, BF)
+
+
 def test_shapes_types_and_strides():
     from flash_pop_b200.token_ops import embedding
     g = torch.Generator(device="cuda").manual_seed(0)

@@ -137,6 +137,50 @@ def test_a_scoring_step_with_the_table_gradient_in_a_graph():
         assert torch.equal(a, b)
 
 
+def test_a_padded_batch_and_the_shortest_sequences():
+    m, tokens = _model(), _tokens(B=3, T=40)
+    table = m.embed.weight
+    whole = m.score(tokens[:2, :25], top=4)
+    want = torch.autograd.grad(whole.logprob.sum(), [table])[0]
+    padded = tokens.clone()
+    padded[:2, 25:] = -1                                         # no token: a zero row, the log probability 0, no gradient
+    s = m.score(padded[:2], top=4)
+    assert bool((s.logprob[:, 24:] == 0).all()) and bool(torch.isfinite(s.entropy).all())
+    assert float((s.logprob[:, :24] - whole.logprob).detach().abs().max()) < 0.1          # (other lengths, other sums: bf16)
+    got = torch.autograd.grad(s.logprob.sum(), [table])[0]
+    assert float((got.double() - want.double()).norm() / want.double().norm()) < 5e-2
+    for T in (0, 1):
+        s = m.score(tokens[:, :T], top=2)
+        assert s.logprob.shape == (3, 0) and s.top_tokens.shape == (3, 0, 2)
+    assert m.score(tokens[:, :2]).logprob.shape == (3, 1)
+
+
+def test_calls_on_two_streams_at_once():
+    from flash_pop_b200 import layer_ops, token_ops
+    g = torch.Generator(device="cuda").manual_seed(0)
+    z, t = torch.randn(64, 20011, generator=g, device="cuda").to(BF).requires_grad_(True), torch.randint(0, 20011, (64,), generator=g, device="cuda")
+    w, ids = torch.randn(3000, 320, generator=g, device="cuda").to(BF).requires_grad_(True), torch.randint(0, 3000, (20000,), generator=g, device="cuda")
+    q = torch.randn(2, 300, 4, 64, generator=g, device="cuda").to(BF).requires_grad_(True)
+    weight, seed = torch.rand(64, device="cuda", requires_grad=True), torch.tensor([9], device="cuda")
+
+    def work():
+        s = token_ops.token_scores(z, t, 20)
+        y = layer_ops.dropout(token_ops.embedding(ids, w, 2.0), 0.1, seed)
+        a, b = layer_ops.qk_norm_rotary(q, q, weight, None, None)
+        return [s.logprob.detach(), s.top_tokens, *torch.autograd.grad([s.entropy.sum(), y.float().sum(), (a + b).float().sum()], [z, w, q, weight])]
+
+    want = work()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    torch.cuda.synchronize()
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(work())
+    torch.cuda.synchronize()
+    for r in got:
+        assert all(torch.equal(a, b) for a, b in zip(r, want))
+
+
 def test_options_are_off_by_default_and_other_layers_take_them():
     import flash_pop_b200 as fp
     from flash_pop_b200.layer_ops import CounterDropout

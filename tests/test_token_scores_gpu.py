@@ -126,6 +126,24 @@ def test_masks_ties_and_extremes(V, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("N,V", [(2100, 9001), (1100, 20000), (2048, 257)])
+def test_many_rows_with_masks_and_ties_among_them(N, V, dtype):
+    """Rows by the thousand run with fewer threads each; masked, constant and rising ones among them take the longer ways."""
+    z, t = _logits(N, V, dtype, N + V)
+    z[::7] = -math.inf
+    z[::14, V // 2:V // 2 + 9] = 1.0                              # nine tokens left, of one value
+    z[1::50] = torch.finfo(dtype).min
+    z[1::100, ::3] = -2.0
+    z[2::60] = 0.5
+    z[3::70] = torch.arange(V, device="cuda").to(dtype)
+    z[4::90, 3] = math.nan
+    z[5::80, V - 200:] = -math.inf                               # a masked end
+    z[6::65, :V - 40] = -math.inf                                # the last forty left
+    for top in (0, 8, 32):
+        _check(z, t, top, grad=top == 8)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_not_a_number_and_infinity_stay_in_their_rows(dtype):
     for V in (300, 40000):
         z, t = _logits(6, V, dtype, 1)
@@ -213,7 +231,7 @@ def test_rows_beyond_32_bits():
     leaf = z.requires_grad_(True)
     s = token_scores(leaf, t, 2)
     assert s.top_tokens[-1].tolist() == [31999, 0] and s.top_tokens[-2].tolist() == [0, 1]
-    assert abs(float(s.logprob[-2]) + math.log(V)) < 1e-5
+    assert abs(float(s.logprob[-2].detach()) + math.log(V)) < 1e-5
     (d,) = torch.autograd.grad(s.logprob.sum(), [leaf])
     p = math.exp(9) / (math.exp(9) + V - 1)
     assert abs(float(d[-1, 31999]) - (1 - p)) < 2.0 ** -8 and abs(float(d[-1, 0]) + p / math.exp(9)) < 1e-6
