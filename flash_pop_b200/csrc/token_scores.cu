@@ -605,13 +605,15 @@ template <typename T, int NT> cudaError_t scores(const ScoreParams& p, cudaStrea
 template <typename T> cudaError_t scores(ScoreParams p, cudaStream_t stream) {
   const int64_t vectors = p.V / (16 / sizeof(T));
   p.split = 1;
-  // Few threads a row where rows are many: what a row costs beside its elements (joins, ranks, barriers) grows with them.  16384
-  // x 32000 bf16, sums: 64 threads 184 us, 128 188, 256 205; with 8 alternatives 281, 275, 320, with 32 498, 393, 430.
+  // Few threads a row where rows are many: what a row costs beside its elements (joins, ranks, barriers) grows with them.  32000 bf16
+  // logits a row, 8 alternatives: 16384 rows with 64, 128 and 256 threads 283, 268 and 320 us, 1024 rows 39, 31 and 33, 300 rows
+  // 29, 20 and 17; a short row gets what holds it in one round of loads.
   if (vectors <= 32 * N && p.top <= FEW) return scores<T, 32>(p, stream);
-  if (vectors <= 64 * N || (p.rows >= 2048 && !p.top)) return scores<T, 64>(p, stream);
-  if (vectors <= 128 * N || p.rows >= 1024) return scores<T, 128>(p, stream);
-  // Few rows: a row over a cluster of CTAs, a vector a thread at least, up to four CTAs an SM.
-  while (p.split < MAX_SPLIT && p.rows * p.split * 2 <= 592 && vectors >= 256 * 2 * p.split) p.split *= 2;
+  if (vectors <= 64 * N) return scores<T, 64>(p, stream);
+  if (vectors <= 128 * N || p.rows >= 592) return scores<T, 128>(p, stream);
+  // Very few rows: a row over a cluster of CTAs, a vector a thread at least, two CTAs an SM at most.  One CTA a row, two, four and eight:
+  // 16 rows 12.3, 12.3, 12.3 and 12.3 us (sums alone 10.2, 10.2, 8.2, 8.2), 64 rows 13.3, 12.3, 12.3 and 14.3, 148 rows 14, 14, 18 and 25.
+  while (p.split < MAX_SPLIT && p.rows * p.split * 2 <= 256 && vectors >= 256 * 2 * p.split) p.split *= 2;
   return scores<T, 256>(p, stream);
 }
 
@@ -717,8 +719,8 @@ template <typename T> cudaError_t scores_grad(const ScoreGradParams& p, cudaStre
   if (vectors <= 32 * 8) return scores_grad<T, 32>(p, 1, stream);
   if (vectors <= 64 * 8) return scores_grad<T, 64>(p, 1, stream);
   if (vectors <= 128 * 8) return scores_grad<T, 128>(p, 1, stream);
-  int split = 1;                                                          // few rows: shares of a row
-  while (split < 64 && p.rows * split * 2 <= 1184 && vectors >= 256 * 2 * split) split *= 2;
+  int split = 1;                   // few rows: shares of a row (16 rows of 32000 bf16: 10.2 us whole, 6.1 in four shares or more, 300 rows 14.3 and 12.3)
+  while (split < 16 && p.rows * split * 2 <= 1184 && vectors >= 256 * 2 * split) split *= 2;
   return scores_grad<T, 256>(p, split, stream);
 }
 
