@@ -710,7 +710,9 @@ namespace {
 int check_qk_norm(int32_t B, int32_t T, int32_t Hq, int32_t Hk, int32_t d, int32_t dtype, const float* w_q, const float* w_k,
                   const float* phasors, int64_t phasor_stride_b) {
   if (B < 0 || T < 0 || Hq < 0 || Hk < 0 || d <= 0 || d % 8 || d > 256) return FPB_ERR_BAD_SHAPE;
-  if (Hq >= (1 << 15) || Hk >= (1 << 15) || (int64_t)B * T * (Hq > Hk ? Hq : Hk) >= (1ll << 31) || (int64_t)B * T >= (1ll << 31)) return FPB_ERR_TOO_LARGE;
+  // (the kernel's token indexes go up to a stretch of tokens past T in 32 bits)
+  if (Hq >= (1 << 15) || Hk >= (1 << 15) || (int64_t)B * T * (Hq > Hk ? Hq : Hk) >= (1ll << 31) || (int64_t)B * T >= (1ll << 31) - (1 << 16))
+    return FPB_ERR_TOO_LARGE;
   if (!dtype_ok(dtype)) return FPB_ERR_BAD_DTYPE;
   if ((uintptr_t)w_q % 16 || (uintptr_t)w_k % 16 || (uintptr_t)phasors % 16 || phasor_stride_b % 2 || phasor_stride_b < 0) return FPB_ERR_BAD_STRIDE;
   return FPB_OK;

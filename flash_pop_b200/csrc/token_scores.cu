@@ -405,7 +405,8 @@ template <typename T, int NT> __device__ __noinline__ void careful_candidates(co
     if (!(most < bound)) push<T, NT>(row, tile, first, end, bound, sh);
     __syncthreads();
     if (sh.found > CANDIDATES) {
-      // no room: the `top` best that earlier tiles left, and this tile's
+      // No room: the `top` best that earlier tiles left, and this tile's.  (The first `top` places of `best` are the CTA's own even
+      // where other CTAs' lists come in behind them.)
       __syncthreads();
       rank_keys<NT>(sh.candidate, kept, top, [&](uint64_t key, int larger) { sh.best[larger] = key; });
       __syncthreads();

@@ -24,6 +24,7 @@ def test_qk_norm_entry_points(handle):
         B, T, Hq, Hk, d, dt, 1e-6, w, None, ph, step, q, SEQ, SEQ, SEQ, None)
     assert fwd(d=12) == fwd(d=264) == fwd(d=0) == fwd(B=-1) == SHAPE
     assert fwd(dt=7) == DTYPE and fwd() == NULL
+    assert fwd(T=(1 << 31) - 100, Hq=1, Hk=1) == fwd(B=1 << 16, T=1 << 15) == fwd(Hq=1 << 15) == LARGE
     assert fwd(w=ctypes.c_void_p(4)) == fwd(ph=ctypes.c_void_p(8)) == fwd(ph=ctypes.c_void_p(16), step=1) == STRIDE
     assert fwd(q=_lib._Seq(0x1008, 128, 32, 16)) == STRIDE
     bwd = lambda scratch, q=SEQ, **kw: handle.fpb_qk_norm_rotary_bwd(0, 4, 2, 2, 16, 0, 1e-6, None, None, None, 0, q, q, q, q, q, q, None, None, scratch, None)
@@ -100,3 +101,24 @@ def test_refused_arguments(anywhere):
     ):
         with pytest.raises(ValueError):
             call()
+
+
+def test_layers_take_the_options_and_refuse_what_the_norms_cannot():
+    import flash_pop_b200 as fp
+    cpu = dict(num_heads=2, head_dim_v=16, dim_feedforward=32, device="cpu", dtype=torch.float32)
+    net = fp.RetNetDecoder(fp.RetNetDecoderLayer.Config(**cpu, qk_norm=True, counter_dropout=True), 1)
+    names = {n for n in net.state_dict() if "norm_weight" in n}
+    assert names == {"layers.0.retention.q_norm_weight", "layers.0.retention.k_norm_weight"}
+    assert net.layers[0].retention.q_norm_weight.shape == (16,) and type(net.layers[0].dropout) is layer_ops.CounterDropout
+    plain = fp.RetNetDecoder(fp.RetNetDecoderLayer.Config(**cpu), 1)
+    assert not [n for n in plain.state_dict() if "norm_weight" in n] and type(plain.layers[0].dropout) is torch.nn.Dropout
+    with pytest.raises(ValueError, match="multiple of 8"):
+        fp.RetNetDecoder(fp.RetNetDecoderLayer.Config(**cpu, head_dim_qk=12, qk_norm=True), 1)
+
+
+def test_counter_dropout_without_anything_to_drop_needs_no_device():
+    x, r = torch.randn(3, 4), torch.randn(3, 4)
+    m = layer_ops.CounterDropout(0.0)
+    assert m(x) is x and torch.equal(m(x, r), r + x)
+    m = layer_ops.CounterDropout(0.5).eval()
+    assert m(x) is x and not m.active() and "p=0.5" in repr(m)
