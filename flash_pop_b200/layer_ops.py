@@ -124,6 +124,7 @@ class QKNormRotary(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dyq, dyk):
         q, k, q_weight, k_weight, phasors = ctx.saved_tensors
+        _lib.native().capturable()
         B, T, Hq, d = q.shape
         Hk = k.size(2)
         dyq, dyk = _aligned(dyq.to(q.dtype), 16), _aligned(dyk.to(q.dtype), 16)
@@ -180,6 +181,7 @@ class Dropout(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         (seed,) = ctx.saved_tensors
+        _lib.native().capturable()
         return _drop(dy, ctx.p, seed, None) if ctx.needs_input_grad[0] else None, dy if ctx.needs_input_grad[1] else None, None, None
 
 

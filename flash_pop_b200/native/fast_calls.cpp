@@ -12,12 +12,14 @@
 #include <ATen/ATen.h>
 #include <ATen/core/TensorBody.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/DynamicTypes.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_function.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -534,6 +536,21 @@ template <typename F> PyObject* guarded_call(Py_ssize_t got, Py_ssize_t want, F 
     }
   });
 }
+// The node that runs, in a captured backward pass, hands no gradient to a node made on the default stream (a leaf's, while an eager
+// graph of the leaf lives): the engine would make that stream wait within the capture, which is an error where nothing catches it.
+void may_be_captured() {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  const std::shared_ptr<torch::autograd::Node> node = torch::autograd::get_current_node();
+  if (!node) return;
+  for (size_t i = 0; i < node->num_outputs(); ++i) {
+    const torch::autograd::Edge& to = node->next_edge(i);
+    if (!to.is_valid() || !node->task_should_compute_output(i)) continue;
+    const std::optional<c10::Stream> stream = to.function->stream();
+    TORCH_CHECK(!stream || *stream != c10::cuda::getDefaultCUDAStream(stream->device_index()).unwrap(),
+                "flash_pop_b200: this backward pass is being captured, and one of its gradients belongs to a graph made on the default stream, which no "
+                "capture may touch: release the outputs of the eager calls with the same leaves first, or make them on the capture's stream");
+  }
+}
 // What a backward returns where a graph of it is recorded: a second derivative raises.
 variable_list once(variable_list out, bool graph) {
   if (!graph) return out;
@@ -602,6 +619,7 @@ struct QkNorm : torch::autograd::Function<QkNorm> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const bool graph = at::GradMode::is_enabled();
     at::NoGradGuard no_grad;
+    may_be_captured();
     const variable_list v = ctx->get_saved_variables();
     const Call c(v[0], v[1], v[2], v[3], v[4], ctx->saved_data["eps"].toDouble());
     Place here(c.q);
@@ -650,6 +668,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const bool graph = at::GradMode::is_enabled();
     at::NoGradGuard no_grad;
+    may_be_captured();
     const at::Tensor seed = ctx->get_saved_variables()[0];
     const at::Tensor dx = ctx->needs_input_grad(0) ? run(dense(g[0]), at::Tensor(), ctx->saved_data["p"].toDouble(), seed, true) : at::Tensor();
     return once({dx, ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(1) ? g[0] : at::Tensor(), at::Tensor(), at::Tensor()}, graph);
@@ -704,6 +723,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const bool graph = at::GradMode::is_enabled();
     at::NoGradGuard no_grad;
+    may_be_captured();
     const at::Tensor t = ctx->get_saved_variables()[0];
     const int64_t V = ctx->saved_data["V"].toInt(), D = g[0].size(-1), N = t.numel();
     Place here(g[0]);
@@ -755,6 +775,7 @@ struct Scores : torch::autograd::Function<Scores> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const bool graph = at::GradMode::is_enabled();
     at::NoGradGuard no_grad;
+    may_be_captured();
     const variable_list v = ctx->get_saved_variables();
     const at::Tensor &z = v[0], &t = v[1], &tt = v[4];
     const int64_t V = z.size(-1), rows = t.numel(), top = tt.defined() ? tt.size(-1) : 0;
@@ -811,6 +832,14 @@ PyObject* wanted(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return r;
 }
 
+// capturable() -> (): raises where the node that runs must not be part of a capture
+PyObject* capturable(PyObject*, PyObject* const*, Py_ssize_t n) {
+  return guarded_call(n, 0, []() -> Tensors {
+    may_be_captured();
+    return {};
+  });
+}
+
 // bind(addresses): the C ABI's entry points in the order of `Entry`
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != ENTRIES) { PyErr_SetString(PyExc_TypeError, "wrong number of entry points"); return nullptr; }
@@ -826,7 +855,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(step), FAST(forward), FAST(backward), FAST(suffix_forward), FAST(suffix_backward), FAST(rotary), FAST(gate_forward),
                          FAST(gate_backward), FAST(norm_forward), FAST(norm_backward), FAST(column_sums), FAST(qk_norm_rotary), FAST(dropout),
-                         FAST(embedding), FAST(token_scores), FAST(address), FAST(wanted), FAST(bind), {nullptr, nullptr, 0, nullptr}};
+                         FAST(embedding), FAST(token_scores), FAST(address), FAST(wanted), FAST(capturable), FAST(bind), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "fpb_fast_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

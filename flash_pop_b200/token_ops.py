@@ -50,6 +50,7 @@ class Embedding(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         (ids,) = ctx.saved_tensors
+        _lib.native().capturable()
         V, D, dtype, scale, padding = ctx.of
         N = ids.numel()
         dy = _matrix(dy.to(dtype).reshape(N, D))
@@ -132,6 +133,7 @@ class _TokenScores(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g_logprob, g_entropy, g_top, _):
         logits, tokens, entropy, stats, top_tokens = ctx.saved_tensors
+        _lib.native().capturable()
         if g_logprob is None and g_entropy is None and g_top is None:
             return None, None, None
         V = logits.size(-1)

@@ -109,3 +109,38 @@ def test_forward_mode_gradients_are_not_dropped():
     with fw.dual_level():
         with pytest.raises(RuntimeError):
             token_ops.token_scores(fw.make_dual(z, torch.ones_like(z)), t)
+
+
+@pytest.mark.parametrize("name", ["qk_norm_rotary", "dropout", "embedding", "token_scores"])
+@pytest.mark.parametrize("fast", [True, False])
+def test_a_capture_beside_a_living_eager_graph_of_its_leaves_is_refused(name, fast, monkeypatch):
+    """The engine would make the default stream wait within the capture, an error that ends the process: the operator's node raises
+    before, and the same capture works once the eager outputs are gone."""
+    from flash_pop_b200 import layer_ops, token_ops
+    if not fast:                                                   # the operators' Python nodes, with the extension's check
+        for module in (layer_ops, token_ops):
+            for f in ("qk_norm_rotary", "dropout", "embedding", "token_scores"):
+                if hasattr(module, f):
+                    monkeypatch.setattr(module._lib.native(), f, lambda *a: None)
+    inputs, call = _calls()[name]
+    leaves = [t.detach().clone().requires_grad_(True) for t in inputs]
+
+    def step():
+        ends = [t for t in call(*leaves) if t is not None and t.is_floating_point()]
+        return ends, lambda: torch.autograd.grad(ends, leaves, [torch.ones_like(t) for t in ends], retain_graph=True)
+
+    eager, grads = step()
+    want = grads()
+    torch.cuda.synchronize()
+    refused, graph, pool = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph(), torch.cuda.graph_pool_handle()
+    with torch.cuda.graph(refused, pool=pool):
+        ends, again = step()
+        with pytest.raises(RuntimeError, match="release the outputs of the eager calls"):
+            again()
+    del eager, grads, ends, again
+    with torch.cuda.graph(graph, pool=pool):
+        ends, again = step()
+        got = again()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want, strict=True))
