@@ -233,10 +233,9 @@ struct ScoreParams {
   int32_t V, top, split;                            // CTAs (of a cluster) that share a row
 };
 
-constexpr int N = 4, U = 8;           // vectors of a thread: in flight at a time, and in a tile that is looked at more closely
+constexpr int N = 4;                  // vectors of a thread in flight at a time, a tile
 constexpr int RECORDS = 512, CANDIDATES = 256, MAX_EDGES = 14, MAX_SPLIT = 8, FEW = 20;
 
-typedef Vectors<U> Tile;
 template <int WARPS> struct Sums {
   Stats parts[WARPS];
   Stats shares[MAX_SPLIT];            // of a row's CTAs, in the first one
@@ -263,78 +262,6 @@ template <int NT, typename F> __device__ __forceinline__ void rank_keys(const ui
     }
     if (larger < top && key) to(key, larger);
   }
-}
-
-// Candidates of a tile where more elements than there is room for reach the bound (masked or constant rows): the tile's k-th
-// largest value exactly, by bisection over its elements; all above it, and of its equals the first ones.  They go behind the
-// `kept` candidates of earlier tiles.
-template <typename T, int NT> __device__ __noinline__ void exact_candidates(const Row<T> row, const Tile tile, int first, int end, int top, int kept,
-                                                                            Shared<NT / 32>& sh) {
-  constexpr int SHIFT = sizeof(T) == 2 ? 16 : 0, WARPS = NT / 32;
-  const uint4 (&r)[U] = tile.r;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  auto total = [&](int n) {
-    n = (int)__reduce_add_sync(ALL, (unsigned)n);
-    __syncthreads();
-    if (lane == 0) sh.count[warp] = (uint32_t)n;
-    __syncthreads();
-    int all = 0;
-    for (int w = 0; w < WARPS; ++w) all += (int)sh.count[w];
-    return all;
-  };
-  auto order = [&](int j, int e) { return order_of(element<T>(r[j], e)) >> SHIFT; };
-  auto here = [&](int j) { return first + j * NT + (int)threadIdx.x < end; };
-  auto at_or_above = [&](uint32_t bound) {
-    int n = 0;
-#pragma unroll
-    for (int j = 0; j < U; ++j)
-#pragma unroll
-      for (int e = 0; e < Row<T>::E; ++e) n += here(j) && order(j, e) >= bound;
-    return total(n);
-  };
-  uint32_t lo = 0, hi = 0xffffffffu >> SHIFT;
-  while (lo < hi) {
-    const uint32_t mid = lo + (hi - lo) / 2 + 1;
-    if (at_or_above(mid) >= top) lo = mid; else hi = mid - 1;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) sh.found = 0;
-  __syncthreads();
-  uint64_t* to = sh.candidate + kept;
-#pragma unroll
-  for (int j = 0; j < U; ++j)
-#pragma unroll
-    for (int e = 0; e < Row<T>::E; ++e)
-      if (here(j) && order(j, e) > lo) to[atomicAdd(&sh.found, 1)] = rank_key(element<T>(r[j], e), row.index(first + j * NT + threadIdx.x, e));      // (fewer than top)
-  __syncthreads();
-  int taken = sh.found;
-#pragma unroll
-  for (int j = 0; j < U; ++j) {        // the vectors' order is that of the indices: round by round, thread by thread
-    if (taken >= top) break;
-    unsigned equal = 0;
-#pragma unroll
-    for (int e = 0; e < Row<T>::E; ++e) equal |= (here(j) && order(j, e) == lo ? 1u : 0u) << e;
-    int before = __popc(equal);
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int n = __shfl_up_sync(ALL, before, o);
-      if (lane >= o) before += n;
-    }
-    const int all = total(lane == 31 ? before : 0);
-    before -= __popc(equal);
-    for (int w = 0; w < warp; ++w) before += (int)sh.count[w];
-#pragma unroll
-    for (int e = 0; e < Row<T>::E; ++e) {
-      if (equal >> e & 1) {
-        if (taken + before < top) to[taken + before] = rank_key(element<T>(r[j], e), row.index(first + j * NT + threadIdx.x, e));
-        ++before;
-      }
-    }
-    taken += all;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) sh.found = kept + min(taken, top);
-  __syncthreads();
 }
 
 // The maxima of the parts that the tiles seen are cut into, 32 or, where more than FEW alternatives are wanted, 64; one or two a lane
@@ -386,37 +313,92 @@ template <typename T, int NT, int N> __device__ __forceinline__ void push(const 
   }
 }
 
-// The candidates of a row where the bound let too many through (masked, constant or rising rows): a bound for every tile, and
-// the tile's exact choice where that does not help either.
-template <typename T, int NT> __device__ __noinline__ void careful_candidates(const Row<T> row, int begin, int end, int top, Shared<NT / 32>& sh) {
+// The candidates of a row where the bound let too many through (constant, rising or oddly masked rows): the top-th largest of its
+// vectors' elements exactly, a digit of its order at a time from counts of the digits; all above it, and of its equals the first ones.
+// In the kernel and with few registers: as a function of its own with tiles in registers it cost the rows that never come here 7 %
+// (16384 rows of 32000 bf16 logits, 8 alternatives) and 16 rows 2 of 12 us.
+template <typename T, int NT> __device__ __forceinline__ void exact_candidates(const Row<T>& row, int begin, int end, int top, Shared<NT / 32>& sh) {
+  constexpr int SHIFT = sizeof(T) == 2 ? 16 : 0, E = Row<T>::E, WARPS = NT / 32, DIGITS = 256;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int* count = reinterpret_cast<int*>(sh.record);                          // of the digits; then the digit, and how many are above it
+  const uint4* from = row.base();
+  uint32_t key = 0;
+  int need = top;                                                          // of those whose upper digits are the key's
+  for (int s = 32 - SHIFT - 8; s >= 0; s -= 8) {
+    __syncthreads();
+    for (int d = threadIdx.x; d < DIGITS; d += NT) count[d] = 0;
+    __syncthreads();
+#pragma unroll 2
+    for (int v = begin + threadIdx.x; v < end; v += NT) {
+      const uint4 r = from[v];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const uint32_t o = order_of(element<T>(r, e)) >> SHIFT >> s;
+        if (o >> 8 == key) atomicAdd(&count[o & 255], 1);
+      }
+    }
+    __syncthreads();
+    if (warp == 0) {                                                       // a lane's eight digits, the largest ones in lane 0
+      int all = 0;
+#pragma unroll
+      for (int d = 0; d < 8; ++d) all += count[DIGITS - 1 - 8 * lane - d];
+      int upto = all;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int n = __shfl_up_sync(ALL, upto, o);
+        if (lane >= o) upto += n;
+      }
+      if (upto - all < need && need <= upto) {
+        int above = upto - all, d = DIGITS - 1 - 8 * lane;
+        while (above + count[d] < need) above += count[d--];
+        count[DIGITS] = d;
+        count[DIGITS + 1] = above;
+      }
+    }
+    __syncthreads();
+    key = key << 8 | (uint32_t)count[DIGITS];
+    need -= count[DIGITS + 1];
+  }
   __syncthreads();
   if (threadIdx.x == 0) sh.found = 0;
-  uint32_t least = 0;
-  int kept = 0;
-  for (int first = begin, parity = 0; first < end; first += U * NT, parity ^= 1) {
-    Tile tile;
-    row.template read<NT>(tile, first, end);
-    const float most = largest_of<T, false>(tile, (end - first - (int)threadIdx.x + NT - 1) / NT);
-    Parts parts;
-    add_maxima<NT>(parts, most, top <= FEW, sh.group[parity]);
-    if (NT == 32) __syncthreads();
-    least = max(least, kth(parts, top));
-    const float bound = value_of(least);
-    if (!(most < bound)) push<T, NT>(row, tile, first, end, bound, sh);
-    __syncthreads();
-    if (sh.found > CANDIDATES) {
-      // No room: the `top` best that earlier tiles left, and this tile's.  (The first `top` places of `best` are the CTA's own even
-      // where other CTAs' lists come in behind them.)
-      __syncthreads();
-      rank_keys<NT>(sh.candidate, kept, top, [&](uint64_t key, int larger) { sh.best[larger] = key; });
-      __syncthreads();
-      kept = min(kept, top);
-      if ((int)threadIdx.x < kept) sh.candidate[threadIdx.x] = sh.best[threadIdx.x];
-      exact_candidates<T, NT>(row, tile, first, end, top, kept, sh);
+  __syncthreads();
+#pragma unroll 2
+  for (int v = begin + threadIdx.x; v < end; v += NT) {
+    const uint4 r = from[v];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float z = element<T>(r, e);
+      if (order_of(z) >> SHIFT > key) sh.candidate[atomicAdd(&sh.found, 1)] = rank_key(z, row.index(v, e));      // (fewer than top)
     }
-    kept = sh.found;
-    __syncthreads();
   }
+  for (int first = begin, taken = 0; first < end && taken < need; first += NT) {                                  // the equals, in order
+    const int v = first + threadIdx.x;
+    const uint4 r = from[min(v, end - 1)];
+    unsigned equal = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) equal |= (v < end && order_of(element<T>(r, e)) >> SHIFT == key ? 1u : 0u) << e;
+    int before = __popc(equal);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int n = __shfl_up_sync(ALL, before, o);
+      if (lane >= o) before += n;
+    }
+    __syncthreads();
+    if (lane == 31) sh.count[warp] = (uint32_t)before;
+    __syncthreads();
+    before += taken - __popc(equal);
+    for (int w = 0; w < WARPS; ++w) {
+      if (w < warp) before += (int)sh.count[w];
+      taken += (int)sh.count[w];
+    }
+    for (; equal && before < need; equal &= equal - 1, ++before) {
+      const int e = __ffs(equal) - 1;
+      sh.candidate[top - need + before] = rank_key(element<T>(r, e), row.index(v, e));
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) sh.found = top;
+  __syncthreads();
 }
 
 // now, wherever the value is used
@@ -543,7 +525,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) scores_kernel(const __grid_cons
       found = sh.found;
       if (found < p.top && there > 4 * p.top) found = CANDIDATES + 1;
     }
-    if (records > RECORDS || found > CANDIDATES) careful_candidates<T, NT>(row, begin, end, p.top, sh);
+    if (records > RECORDS || found > CANDIDATES) exact_candidates<T, NT>(row, begin, end, p.top, sh);
     if (share == 0 && row.edges()) {
       __syncthreads();                               // (all have read `found`)
       if (has_edge && order_of(edge) >= least) sh.candidate[atomicAdd(&sh.found, 1)] = rank_key(edge, row.edge(threadIdx.x));
