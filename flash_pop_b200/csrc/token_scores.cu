@@ -592,14 +592,15 @@ template <typename T, int NT> cudaError_t scores(const ScoreParams& p, cudaStrea
 template <typename T> cudaError_t scores(ScoreParams p, cudaStream_t stream) {
   const int64_t vectors = p.V / (16 / sizeof(T));
   p.split = 1;
-  // Few threads a row where rows are many: what a row costs beside its elements (joins, ranks, barriers) grows with them.  32000 bf16
-  // logits a row, 8 alternatives: 16384 rows with 64, 128 and 256 threads 283, 268 and 320 us, 1024 rows 39, 31 and 33, 300 rows
-  // 29, 20 and 17; a short row gets what holds it in one round of loads.
+  // Few threads a row where rows are many: what a row costs beside its elements (joins, ranks, barriers) grows with them.  bf16 logits, 8
+  // alternatives, with 64, 128 and 256 threads: 16384 rows of 32000 209, 223 and 264 us, 8192 rows 120 and 123, 1024 rows 31, 27 and 29, 300
+  // rows 22, 16 and 16; 64 and 128: 16384 rows of 4000 74 and 82, 2048 rows equal, 4096 rows of 128000 211 and 193, and without
+  // alternatives 16384 rows of 8192 61 and 68, 8192 rows of 32000 108 and 103.  A short row gets what holds it in one round of loads.
   if (vectors <= 32 * N && p.top <= FEW) return scores<T, 32>(p, stream);
-  if (vectors <= 64 * N) return scores<T, 64>(p, stream);
+  if (vectors <= 64 * N || (p.rows >= 2048 && vectors <= 64 * N * (p.top ? 16 : 4))) return scores<T, 64>(p, stream);
   if (vectors <= 128 * N || p.rows >= 592) return scores<T, 128>(p, stream);
   // Very few rows: a row over a cluster of CTAs, a vector a thread at least, two CTAs an SM at most.  One CTA a row, two, four and eight:
-  // 16 rows 12.3, 12.3, 12.3 and 12.3 us (sums alone 10.2, 10.2, 8.2, 8.2), 64 rows 13.3, 12.3, 12.3 and 14.3, 148 rows 14, 14, 18 and 25.
+  // 16 rows 12.3, 12.3, 10.2 and 10.2 us (sums alone 10.2, 10.2, 8.2, 8.2), 64 rows 12.3, 12.3, 12.3 and 14.3, 148 rows 12, 14, 18 and 22.
   while (p.split < MAX_SPLIT && p.rows * p.split * 2 <= 256 && vectors >= 256 * 2 * p.split) p.split *= 2;
   return scores<T, 256>(p, stream);
 }

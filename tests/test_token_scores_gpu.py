@@ -144,6 +144,28 @@ def test_many_rows_with_masks_and_ties_among_them(N, V, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("N,V", [(2048, 16003), (16, 16003), (200, 40010)])
+def test_rows_where_the_choice_is_by_digits(N, V, dtype):
+    """Rows where more elements reach the bound than there is room for: ties and neighbours at each digit, both signs, every split."""
+    z, t = _logits(N, V, dtype, N + V + 1)
+    i = torch.arange(V, device="cuda")
+    unit = torch.finfo(dtype).eps
+    special = [-(V - i) / 64.0,                                   # rising, negative
+               torch.where(i % 29 == 5, 3.0, -1.0),               # a few hundred equal largest
+               torch.where(i % 29 == 5, -3.0, -5.0) + (i == V - 7) * 1.0,      # negative ones, and one above them
+               1.0 + unit * (i * 7 % 113 % 5),                    # neighbours of one another
+               -1.0 - unit * (i * 7 % 113 % 5),
+               torch.where(i > V // 2, i / 64.0, 0.0),            # rising from the middle on
+               torch.where(i < 700, i / 8.0 - 50.0, -70.0),       # a rising start
+               torch.where(i == V - 9, math.nan, i / 64.0),
+               torch.where(i % 2 == 0, 2.0 ** -130, -(2.0 ** -130))]           # below the normal numbers
+    for r, row in enumerate(special):
+        z[r::len(special) + 2] = row.to(dtype)
+    for top in (1, 8, 31):
+        _check(z, t, top, grad=False)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_not_a_number_and_infinity_stay_in_their_rows(dtype):
     for V in (300, 40000):
         z, t = _logits(6, V, dtype, 1)
