@@ -438,8 +438,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) scores_kernel(const __grid_cons
   // `top` parts of the tiles seen reach the top-th largest of the parts' maxima: so many elements do, and of any order of the
   // elements not many more are to be expected (of one tile 32 ln(32 / (32 - top))).  The bound is taken again when as many
   // tiles have passed as before: it lets about as many through from one time to the next.  Maxima of all tiles, the bound at the tiles 0, 3,
-  // 7, 15, ...: 32000 bf16 logits, 1, 8 and 32 alternatives 209, 243 and 331 us; at the tile 1 as well 212, 250 and 340, and with maxima of
-  // those tiles alone 213, 262 and 405; at 0, 3 and 15 (8 and 32) 248 and 374, at 0, 4, 12, ... 244 and 354.
+  // 7, 15, ...: 16384 rows of 32000 bf16 logits, 128 threads and 1, 8 and 32 alternatives 209, 243 and 331 us (193, 223 and 307 since the exact
+  // choice is no call); at the tile 1 as well 212, 250 and 340, and with maxima of those tiles alone 213, 262 and 405; at 0, 3 and 15 (8
+  // and 32) 248 and 374, at 0, 4, 12, ... 244 and 354.
   float mine = -INFINITY;                            // a thread's maximum of all tiles so far (a NaN only lowers the bound)
   uint32_t least = order_of(-INFINITY);              // the bound's order; `bound`: the smallest value that counts
   bool masked = true;
