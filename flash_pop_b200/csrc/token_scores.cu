@@ -87,20 +87,25 @@ template <typename T> __device__ __forceinline__ float largest(const uint4& r) {
 
 // ---- sums -----------------------------------------------------------------------------------------------------------
 // In powers of two: with L = log2 e and c = m L rounded, x = 2^(z L - c) is one rounding of the exponent (a fused product) and one
-// exponential; that c is not m L exactly shifts all exponents alike and is put right once, in the logarithm of the sum.  Where
-// c could overflow, and where a mask has filled what is left with huge negative numbers, x = 2^((z - m) L).
-constexpr float LARGEST = 2e38f, SMALLEST = -1e29f, FILL = -9e29f;
-__device__ __forceinline__ bool ordinary(float m) { return m > SMALLEST && m < LARGEST; }
+// exponential; that c is not m L exactly shifts all exponents alike and is put right once, in the logarithm of the sum.  The shift is half a
+// unit in c's last place at most: 2^-4 below |m| = 2^20, but 2^7 and more from |m| = 2^31 on, where 2^shift is 0 or infinite.  So larger
+// maxima (masks of finite numbers among them), and m = -inf, take x = 2^((z - m) L), a rounding more, without a shift.
+constexpr float ORDINARY = 1048576.0f;
+__device__ __forceinline__ bool ordinary(float m) { return fabsf(m) < ORDINARY; }
 __device__ __forceinline__ float origin(float m) { return __fmul_rn(m, LOG2E); }        // c (never fused into what follows)
 __device__ __forceinline__ float exponent(float z, float m) { return ordinary(m) ? fmaf(z, LOG2E, -origin(m)) : (z - m) * LOG2E; }
+// Alternatives' bounds below SMALLEST are those of a masked row; FILL stands for the elements behind a row, which no sum feels.
+constexpr float SMALLEST = -1e29f, FILL = -9e29f;
 
 // running (max, sum of x, sum of x times its exponent); nothing yet, or only -inf: max = -inf, sums 0
 struct Stats {
   float m, s, t;
 };
-// the same sums against another maximum, at least as large
+// the same sums against another maximum, at least as large; either may have a shift, which goes with its exponents
 __device__ __forceinline__ void move_to(Stats& a, float m) {
-  const float d = ordinary(m) && ordinary(a.m) ? __fsub_rn(origin(a.m), origin(m)) : (a.m - (m == -INFINITY ? 0.0f : m)) * LOG2E;
+  const float base = m == -INFINITY ? 0.0f : m;
+  const float d = ordinary(a.m) ? (ordinary(m) ? __fsub_rn(origin(a.m), origin(m)) : -fmaf(m, LOG2E, -origin(a.m)))
+                                : (ordinary(m) ? fmaf(a.m, LOG2E, -origin(m)) : (a.m - base) * LOG2E);
   const float y = at_least(d), c = exp2_of(y);
   a.t = c * fmaf(a.s, y, a.t);
   a.s *= c;

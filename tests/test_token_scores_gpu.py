@@ -281,3 +281,65 @@ def test_same_bits_twice_and_in_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, want))
+
+
+FILLS = [-1e5, -1e9, -5e9, -1e10, -1e12, -1e15, -1e20, -1e25]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("V", [100, 5000, 33000, 100001])
+def test_finite_masks_of_any_size(V, dtype):
+    """A masked start, a masked end, all masked but a few, and all: whatever number stands for the mask."""
+    z, t = _logits(4 * len(FILLS), V, dtype, V + 11)
+    for i, fill in enumerate(FILLS):
+        z[4 * i, :V // 2] = z[4 * i + 1, V // 2:] = z[4 * i + 3] = fill
+        kept = z[4 * i + 2, V // 3:V // 3 + 4].clone()
+        z[4 * i + 2] = fill
+        z[4 * i + 2, V // 3:V // 3 + 4] = kept
+    t[::4] = V - 1                                               # one given token that is not masked, of the others some are
+    for top in (0, 3, 20, 32):
+        _check(z, t, top)
+
+
+def _large_rows(V, dtype):
+    """Rows whose largest element is huge, or that pass from one size to another."""
+    i = torch.arange(V, device="cuda", dtype=torch.float64)
+    g = torch.Generator(device="cuda").manual_seed(V)
+    noise = torch.randn(V, generator=g, device="cuda", dtype=torch.float64)
+    rows = []
+    for m in (3e9, 5e9, 1e10, 1e12, 1e20, 1e38):
+        for sign in (1, -1):
+            rows += [torch.full_like(i, sign * m),                                   # all equal
+                     sign * m * (1 + torch.finfo(dtype).eps * (i % 3)),              # neighbours of one another
+                     torch.where(i == V // 2, sign * m, 3 * noise if sign > 0 else 2 * sign * m)]      # one above the others
+    for edge in (2.0 ** 18, 2.0 ** 20, 2.0 ** 24):                                  # up and down across sizes where fewer bits are left
+        step = edge * torch.finfo(dtype).eps
+        for sign in (1, -1):
+            rows += [sign * edge + (i - V // 2) * step, sign * edge - (i - V // 2) * step, sign * edge + (i % 7 - 3) * step]
+        rows.append(torch.where(i % 2 == 0, edge, -edge) + noise)
+    rows += [noise - 5e9, torch.where(i < V // 2, -2.0 ** 19 - i, 2.0 ** 21), torch.where(i < V // 2, -2.0 ** 21 - i, 2.0 ** 19),
+             torch.where(i < V // 2, -2.0 ** 21 - i, noise), torch.where(i < V // 2, -2.0 ** 20 + noise, -2.0 ** 20 - 1 + noise)]
+    return torch.stack(rows).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("V", [7, 100, 5000, 33000, 100001])
+def test_finite_rows_of_any_size(V, dtype):
+    z = _large_rows(V, dtype)
+    assert bool(z.isfinite().all())
+    t = torch.randint(0, V, (z.size(0),), generator=torch.Generator(device="cuda").manual_seed(9), device="cuda")
+    t[::2] = z[::2].float().argmax(1)
+    for top in (0, min(V, 5), min(V, 32)):
+        _check(z, t, top)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_many_rows_of_any_size(dtype):
+    V = 9001
+    rows = _large_rows(V, dtype)
+    z, t = _logits(2100, V, dtype, 12)
+    z[:40 * rows.size(0)] = rows.repeat(40, 1)[:2100]
+    z[-300::8, :V // 2] = -1e10
+    z[-299::8, 9:] = -5e9
+    for top in (0, 8):
+        _check(z, t, top)
