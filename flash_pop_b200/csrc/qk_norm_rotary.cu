@@ -78,6 +78,10 @@ __device__ __forceinline__ Eight rotate(const Eight& x, const Pair (&c)[2], cons
   return y;
 }
 
+// eight elements of the packed word `w` (two bf16 or one fp32)
+__device__ __forceinline__ void fill8(Raw8<__nv_bfloat16>& r, uint32_t w) { r.a = make_uint4(w, w, w, w); }
+__device__ __forceinline__ void fill8(Raw8<float>& r, uint32_t w) { r.a = r.b = make_uint4(w, w, w, w); }
+
 template <typename T, int L, int HEADS, bool BWD>
 __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 2 : 4) qk_norm_kernel(const __grid_constant__ QkNormParams p) {
   constexpr int GROUPS = THREADS / L;
@@ -86,6 +90,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 2 : 4) qk_norm_kerne
   const SeqView vx = p.x[which], vg = p.dy[which], vo = p.out[which];
   const int group = threadIdx.x / L, lane = threadIdx.x % L, c0 = lane * 8;
   const bool live = c0 < p.d;
+  // What stands for a row that is not there: ones, whose r is finite without eps too, under a gradient of zeros; lanes behind d add nothing.
+  const uint32_t blank = live ? (sizeof(T) == 2 ? 0x3f803f80u : 0x3f800000u) : 0u;
   float f[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) f[e] = live && p.w[which] ? p.w[which][c0 + e] : 1.0f;
@@ -116,7 +122,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 2 : 4) qk_norm_kerne
       float4 u = make_float4(1.0f, 0.0f, 1.0f, 0.0f), v = u;
 #pragma unroll
       for (int j = 0; j < HEADS; ++j) {
-        rx[j] = Raw8<T>{};
+        fill8(rx[j], blank);
         if constexpr (BWD) rg[j] = Raw8<T>{};
         if (here && j < heads) {
           read8(x_at + j * vx.sh, rx[j]);

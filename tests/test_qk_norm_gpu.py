@@ -167,3 +167,14 @@ def test_empty_calls():
         assert yq.shape == q.shape and yk.shape == k.shape
         gq, gw = torch.autograd.grad((yq, yk), [q, w], (torch.ones_like(yq), torch.ones_like(yk)))
         assert gq.shape == q.shape and gw.shape == w.shape and bool(torch.isfinite(gw).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("B,T,Hq,Hk,d", [(1, 3, 1, 1, 8), (2, 77, 5, 3, 40), (1, 33, 7, 1, 64), (1, 19, 3, 5, 200), (3, 21, 17, 16, 256)])
+def test_without_eps(B, T, Hq, Hk, d, dtype):
+    """eps = 0, or one that fp32 does not hold: rows that are not there (odd heads, the last stretch of tokens) leave nothing behind."""
+    g = torch.Generator(device="cuda").manual_seed(T)
+    rnd = lambda *s, t=dtype: torch.randn(*s, generator=g, device="cuda").to(t)
+    q, k, dyq, dyk = rnd(B, T, Hq, d), rnd(B, T, Hk, d), rnd(B, T, Hq, d), rnd(B, T, Hk, d)
+    for eps in (0.0, 1e-60):
+        _check(q, k, 1 + 0.2 * rnd(d, t=F32), 1 + 0.2 * rnd(d, t=F32), _phasors(1, T, d), eps, dyq, dyk)
