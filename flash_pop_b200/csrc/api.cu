@@ -707,9 +707,9 @@ int fpb_cross_entropy_bwd(int64_t rows, int32_t V, int32_t dtype, const void* lo
 }
 
 namespace {
-int check_qk_norm(int32_t B, int32_t T, int32_t Hq, int32_t Hk, int32_t d, int32_t dtype, const float* w_q, const float* w_k,
+int check_qk_norm(int32_t B, int32_t T, int32_t Hq, int32_t Hk, int32_t d, int32_t dtype, float eps, const float* w_q, const float* w_k,
                   const float* phasors, int64_t phasor_stride_b) {
-  if (B < 0 || T < 0 || Hq < 0 || Hk < 0 || d <= 0 || d % 8 || d > 256) return FPB_ERR_BAD_SHAPE;
+  if (B < 0 || T < 0 || Hq < 0 || Hk < 0 || d <= 0 || d % 8 || d > 256 || !(eps >= 0.0f)) return FPB_ERR_BAD_SHAPE;
   // (the kernel's token indexes go up to a stretch of tokens past T in 32 bits)
   if (Hq >= (1 << 15) || Hk >= (1 << 15) || (int64_t)B * T * (Hq > Hk ? Hq : Hk) >= (1ll << 31) || (int64_t)B * T >= (1ll << 31) - (1 << 16))
     return FPB_ERR_TOO_LARGE;
@@ -722,7 +722,7 @@ int check_qk_norm(int32_t B, int32_t T, int32_t Hq, int32_t Hk, int32_t d, int32
 int fpb_qk_norm_rotary_fwd(int32_t B, int32_t T, int32_t Hq, int32_t Hk, int32_t d, int32_t dtype, float eps, const float* w_q,
                            const float* w_k, const float* phasors, int64_t phasor_stride_b, const fpb_seq* q, const fpb_seq* k,
                            const fpb_seq* q_out, const fpb_seq* k_out, fpb_stream_t stream) {
-  FPB_TRY(check_qk_norm(B, T, Hq, Hk, d, dtype, w_q, w_k, phasors, phasor_stride_b));
+  FPB_TRY(check_qk_norm(B, T, Hq, Hk, d, dtype, eps, w_q, w_k, phasors, phasor_stride_b));
   FPB_TRY(check_plain_seq(q, dtype, B, T, Hq, d, 16)); FPB_TRY(check_plain_seq(k, dtype, B, T, Hk, d, 16));
   FPB_TRY(check_plain_seq(q_out, dtype, B, T, Hq, d, 16)); FPB_TRY(check_plain_seq(k_out, dtype, B, T, Hk, d, 16));
   FPB_TRY(check_device());
@@ -739,7 +739,7 @@ int fpb_qk_norm_rotary_bwd(int32_t B, int32_t T, int32_t Hq, int32_t Hk, int32_t
                            const float* w_k, const float* phasors, int64_t phasor_stride_b, const fpb_seq* q, const fpb_seq* k,
                            const fpb_seq* d_yq, const fpb_seq* d_yk, const fpb_seq* d_q, const fpb_seq* d_k, float* d_w_q, float* d_w_k,
                            void* scratch, fpb_stream_t stream) {
-  FPB_TRY(check_qk_norm(B, T, Hq, Hk, d, dtype, w_q, w_k, phasors, phasor_stride_b));
+  FPB_TRY(check_qk_norm(B, T, Hq, Hk, d, dtype, eps, w_q, w_k, phasors, phasor_stride_b));
   FPB_TRY(check_plain_seq(q, dtype, B, T, Hq, d, 16)); FPB_TRY(check_plain_seq(k, dtype, B, T, Hk, d, 16));
   FPB_TRY(check_plain_seq(d_yq, dtype, B, T, Hq, d, 16)); FPB_TRY(check_plain_seq(d_yk, dtype, B, T, Hk, d, 16));
   FPB_TRY(check_plain_seq(d_q, dtype, B, T, Hq, d, 16)); FPB_TRY(check_plain_seq(d_k, dtype, B, T, Hk, d, 16));

@@ -73,7 +73,12 @@ def rotary_qk(q: Tensor, k: Tensor, phasors: Tensor, out_dtype: Optional[torch.d
 
 
 # ---- norms of queries and keys, then the rotation ------------------------------------------------------------------
-def _check_qk_norm(q: Tensor, k: Tensor, q_weight: Optional[Tensor], k_weight: Optional[Tensor], phasors: Optional[Tensor]) -> None:
+def check_qk_norm_eps(eps: float) -> None:
+    if not eps >= 0.0:
+        raise ValueError(f"the norms' eps has to be a number that is not negative; got {eps}")
+
+
+def _check_qk_norm(q: Tensor, k: Tensor, q_weight: Optional[Tensor], k_weight: Optional[Tensor], phasors: Optional[Tensor], eps: float) -> None:
     _lib.require_cuda(q, k, q_weight, k_weight, phasors)
     if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.size(3) != k.size(3):
         raise ValueError(f"q and k: (B, T, heads, d) with the same B, T and d; got {tuple(q.shape)} and {tuple(k.shape)}")
@@ -90,6 +95,7 @@ def _check_qk_norm(q: Tensor, k: Tensor, q_weight: Optional[Tensor], k_weight: O
         raise ValueError(f"phasors: float32 (1 or {q.size(0)}, {q.size(1)}, {d // 2}, 2); got {phasors.dtype} {tuple(phasors.shape)}")
     if any(t is not None and t.device != q.device for t in (k, q_weight, k_weight, phasors)):
         raise ValueError("q, k, the weights and the phasors have to be on one device")
+    check_qk_norm_eps(eps)
 
 
 def _norm_weight(w: Optional[Tensor]) -> Optional[Tensor]:
@@ -102,7 +108,7 @@ def _norm_weight(w: Optional[Tensor]) -> Optional[Tensor]:
 class QKNormRotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, phasors, eps):
-        _check_qk_norm(q, k, q_weight, k_weight, phasors)
+        _check_qk_norm(q, k, q_weight, k_weight, phasors, eps)
         if phasors is not None:
             phasors = phasors.contiguous()
             if phasors.data_ptr() % 16:
@@ -143,7 +149,7 @@ def qk_norm_rotary(q: Tensor, k: Tensor, q_weight: Optional[Tensor], k_weight: O
                    eps: float = 1e-6) -> Tuple[Tensor, Tensor]:
     """RMS norm of every head of q (B, T, Hq, d) and k (B, T, Hk, d), ``x / sqrt(mean(x^2) + eps) * weight``, then the rotation of
     the channel pairs by `phasors` (1 or B, T, d/2, 2) = (cos, sin), fp32 (None: no rotation), in one pass.  The weights
-    (d elements each, None: ones) are shared by the heads; d a multiple of 8, at most 256.  fp32 arithmetic, results in q's dtype.
+    (d elements each, None: ones) are shared by the heads; d a multiple of 8, at most 256; eps not negative (0: a head of zeros gives NaN).  fp32 arithmetic, results in q's dtype.
     No gradient goes to the phasors; the weights' gradients are summed in a fixed order."""
     eps = float(eps)
     fast = _lib.result(_lib.native().qk_norm_rotary(q, k, q_weight, k_weight, phasors, eps))
@@ -151,7 +157,7 @@ def qk_norm_rotary(q: Tensor, k: Tensor, q_weight: Optional[Tensor], k_weight: O
         return fast
     for w in (q_weight, k_weight):
         if w is not None and w.dtype != torch.float32:           # (their gradients go back through the casts)
-            _check_qk_norm(q, k, q_weight, k_weight, phasors)
+            _check_qk_norm(q, k, q_weight, k_weight, phasors, eps)
             q_weight, k_weight = (None if w is None else w.to(torch.float32) for w in (q_weight, k_weight))
     return QKNormRotary.apply(q, k, q_weight, k_weight, None if phasors is None else phasors.detach(), eps)
 

@@ -590,7 +590,7 @@ struct QkNorm : torch::autograd::Function<QkNorm> {
     }
     void check() const {
       NEED(real(q.scalar_type()) && k.scalar_type() == q.scalar_type() && k.device() == q.device() && k.size(0) == B && k.size(1) == T && k.size(3) == d);
-      NEED(d % 8 == 0 && d <= 256 && q.numel() < INT32_MAX && k.numel() < INT32_MAX);
+      NEED(d % 8 == 0 && d <= 256 && eps >= 0.0f && q.numel() < INT32_MAX && k.numel() < INT32_MAX);
       NEED(in_place(q) && aligned(q, 16) && in_place(k) && aligned(k, 16));
       param(wq, d, q); param(wk, d, q);
       if (ph.defined())

@@ -26,8 +26,8 @@ import torch.nn.functional as F
 from torch import Tensor
 
 from flash_pop_b200.fused_retention import cuda_core_kernels, fused_chunk_retention, retention_step
-from flash_pop_b200.layer_ops import (CounterDropout, SwishFeedForward, groupnorm_gate, groupnorm_gate_supported, linear_group, linears_supported,
-                                      norm_in_fp32, qk_norm_rotary)
+from flash_pop_b200.layer_ops import (CounterDropout, SwishFeedForward, check_qk_norm_eps, groupnorm_gate, groupnorm_gate_supported, linear_group,
+                                      linears_supported, norm_in_fp32, qk_norm_rotary)
 from flash_pop_b200.recurrent_state import RecurrentState
 from flash_pop_b200.token_stack import decoder_token
 from flash_pop_b200.xpos_emb import XPos
@@ -138,6 +138,7 @@ class MultiScaleRetention(nn.Module):
         if config.qk_norm:
             if self.head_dim_qk % 8 or self.head_dim_qk > 256:
                 raise ValueError(f"qk_norm needs a head dimension of q and k that is a multiple of 8 and at most 256; got {self.head_dim_qk}")
+            check_qk_norm_eps(config.qk_norm_eps)
             self.q_norm_weight = nn.Parameter(torch.ones(self.head_dim_qk, device=config.device, dtype=torch.float32))
             self.k_norm_weight = nn.Parameter(torch.ones(self.head_dim_qk, device=config.device, dtype=torch.float32))
         self._reset_parameters()

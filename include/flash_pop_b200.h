@@ -335,7 +335,7 @@ int fpb_cross_entropy_bwd(int64_t rows, int32_t V, int32_t dtype, const void* lo
 /*
  * Norms of queries and keys over each head, then the position rotation, in one pass over (B, T, Hq, d) queries and (B, T, Hk, d)
  * keys (d a multiple of 8, at most 256; bf16 or fp32, fp32 arithmetic; tensors and strides 16-byte aligned):
- *   y = R (x r w),  r = 1 / sqrt(mean over d of x^2 + eps)
+ *   y = R (x r w),  r = 1 / sqrt(mean over d of x^2 + eps),  eps >= 0
  * w_q, w_k: d fp32 weights each, 16-byte aligned, NULL: ones.  phasors as fpb_rotary takes them, NULL: no rotation.
  * The backward reads x and d_y, writes d_x and, where d_w_q / d_w_k are given (fp32), the weights' gradients: sums over all rows in a
  * fixed order.  `scratch`: FPB_QK_NORM_SCRATCH(d) device bytes, 16-byte aligned, used during the call only.  The reference

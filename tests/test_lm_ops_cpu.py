@@ -122,3 +122,18 @@ def test_counter_dropout_without_anything_to_drop_needs_no_device():
     assert m(x) is x and torch.equal(m(x, r), r + x)
     m = layer_ops.CounterDropout(0.5).eval()
     assert m(x) is x and not m.active() and "p=0.5" in repr(m)
+
+
+def test_eps_of_the_norms_is_checked(handle, anywhere):
+    fwd = lambda eps: handle.fpb_qk_norm_rotary_fwd(1, 4, 2, 2, 16, 0, eps, None, None, None, 0, SEQ, SEQ, SEQ, SEQ, None)
+    bwd = lambda eps: handle.fpb_qk_norm_rotary_bwd(1, 4, 2, 2, 16, 0, eps, None, None, None, 0, SEQ, SEQ, SEQ, SEQ, SEQ, SEQ, None, None, None, None)
+    for eps in (-1e-6, float("nan"), -float("inf")):
+        assert fwd(eps) == bwd(eps) == SHAPE
+        q = torch.randn(2, 3, 4, 16)
+        with pytest.raises(ValueError, match="eps"):
+            layer_ops.qk_norm_rotary(q, q, None, None, None, eps)
+        import flash_pop_b200 as fp
+        with pytest.raises(ValueError, match="eps"):
+            fp.RetNetDecoder(fp.RetNetDecoderLayer.Config(num_heads=2, head_dim_v=16, dim_feedforward=32, device="cpu", dtype=torch.float32, qk_norm=True,
+                                                          qk_norm_eps=eps), 1)
+    assert fwd(0.0) == NULL and bwd(0.0) == NULL
