@@ -105,6 +105,14 @@ def _norm_weight(w: Optional[Tensor]) -> Optional[Tensor]:
     return w if w.data_ptr() % 16 == 0 else w.clone()
 
 
+def _readable(t: Tensor) -> Tensor:
+    """`t` (B, T, heads, d) as the norms' kernels read it.  (A contiguous tensor may still begin, or have a stride that no element uses, beside
+    the 16-byte boundaries.)"""
+    t = _aligned(t, 16)
+    vec = 16 // t.element_size()
+    return t if t.data_ptr() % 16 == 0 and all(s % vec == 0 for s in t.stride()[:-1]) else t.clone(memory_format=torch.contiguous_format)
+
+
 class QKNormRotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, phasors, eps):
@@ -114,7 +122,7 @@ class QKNormRotary(torch.autograd.Function):
             if phasors.data_ptr() % 16:
                 phasors = phasors.clone()
         q_weight, k_weight = _norm_weight(q_weight), _norm_weight(k_weight)
-        q, k = _aligned(q, 16), _aligned(k, 16)
+        q, k = _readable(q), _readable(k)
         B, T, Hq, d = q.shape
         Hk = k.size(2)
         y_q, y_k = torch.empty((B, T, Hq, d), device=q.device, dtype=q.dtype), torch.empty((B, T, Hk, d), device=q.device, dtype=q.dtype)
@@ -133,7 +141,7 @@ class QKNormRotary(torch.autograd.Function):
         _lib.native().capturable()
         B, T, Hq, d = q.shape
         Hk = k.size(2)
-        dyq, dyk = _aligned(dyq.to(q.dtype), 16), _aligned(dyk.to(q.dtype), 16)
+        dyq, dyk = _readable(dyq.to(q.dtype)), _readable(dyk.to(q.dtype))
         dq, dk = torch.empty((B, T, Hq, d), device=q.device, dtype=q.dtype), torch.empty((B, T, Hk, d), device=q.device, dtype=q.dtype)
         dwq, dwk = (torch.empty(d, device=q.device, dtype=torch.float32) if n else None for n in ctx.needs_input_grad[2:4])
         with torch.cuda.device(q.device):

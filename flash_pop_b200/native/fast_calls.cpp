@@ -565,7 +565,8 @@ at::Tensor dense(const at::Tensor& t) {          // contiguous and 16-byte align
 }
 at::Tensor readable(const at::Tensor& t) {       // rows as the kernels take them, copied if need be
   if (t.numel() == 0 || (in_place(t) && aligned(t, 16))) return t;
-  return dense(t);
+  const at::Tensor c = dense(t);                 // (contiguous as it was, it may keep a stride that no element uses)
+  return aligned(c, 16) ? c : c.clone(at::MemoryFormat::Contiguous);
 }
 // (an absent tensor is no input of a node, nor counted among them)
 typedef std::optional<at::Tensor> Maybe;

@@ -178,3 +178,37 @@ def test_without_eps(B, T, Hq, Hk, d, dtype):
     q, k, dyq, dyk = rnd(B, T, Hq, d), rnd(B, T, Hk, d), rnd(B, T, Hq, d), rnd(B, T, Hk, d)
     for eps in (0.0, 1e-60):
         _check(q, k, 1 + 0.2 * rnd(d, t=F32), 1 + 0.2 * rnd(d, t=F32), _phasors(1, T, d), eps, dyq, dyk)
+
+
+@pytest.mark.parametrize("fast", [True, False])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_contiguous_tensors_that_are_not_aligned(dtype, fast, monkeypatch):
+    from flash_pop_b200 import _lib
+    from flash_pop_b200.layer_ops import qk_norm_rotary
+    if not fast:
+        monkeypatch.setattr(_lib, "native", lambda: _lib._Declines())
+    g = torch.Generator(device="cuda").manual_seed(8)
+    B, T, H, d = 2, 5, 3, 24
+    n = B * T * H * d
+
+    def offset(t, by=1):
+        flat = torch.empty(n + by, device="cuda", dtype=t.dtype)
+        flat[by:] = t.flatten()
+        return flat[by:].view(t.shape)
+
+    q, k, dyq, dyk = (torch.randn(B, T, H, d, generator=g, device="cuda").to(dtype) for _ in range(4))
+    w, ph = torch.rand(d, device="cuda").requires_grad_(True), _phasors(1, T, d)
+    moved = [offset(t) for t in (q, k, dyq, dyk)]
+    assert all(t.is_contiguous() and t.data_ptr() % 16 for t in moved)
+
+    def step(q, k, dyq, dyk):
+        q, k = q.detach().requires_grad_(True), k.detach().requires_grad_(True)
+        y = qk_norm_rotary(q, k, w, w, ph)
+        return [t.detach() for t in y] + list(torch.autograd.grad(y, [q, k, w], (dyq, dyk)))
+
+    want = step(q, k, dyq, dyk)
+    for args in (moved, [moved[0], k, dyq, moved[3]], [q, k, moved[2], dyk]):
+        assert all(torch.equal(a, b) for a, b in zip(step(*args), want, strict=True))
+    ones = [torch.empty_strided((1, T, H, d), (7, H * d, d, 1), device="cuda", dtype=dtype).copy_(t[:1]) for t in (q, k, dyq, dyk)]
+    assert all(t.is_contiguous() and t.stride(0) == 7 for t in ones)                     # an odd stride that no element uses
+    assert all(torch.equal(a, b) for a, b in zip(step(*ones), step(q[:1], k[:1], dyq[:1], dyk[:1]), strict=True))
