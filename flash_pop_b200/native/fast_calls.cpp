@@ -23,6 +23,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include "../../include/flash_pop_b200.h"
 
@@ -189,7 +190,8 @@ template <typename F> int unlocked(F f) {
 template <typename F> PyObject* guarded(Py_ssize_t got, Py_ssize_t want, F body) {
   if (got != want) { PyErr_Format(PyExc_TypeError, "expected %zd arguments, got %zd", want, got); return nullptr; }
   try {
-    if (!entry.step || c10::impl::TorchDispatchModeTLS::any_modes_set()) Py_RETURN_NONE;
+    // (a trace would record the results' allocation and nothing that fills them; an autograd.Function it records as a whole)
+    if (!entry.step || c10::impl::TorchDispatchModeTLS::any_modes_set() || torch::jit::tracer::isTracing()) Py_RETURN_NONE;
     return body();
   } catch (const NotOurs&) {
     Py_RETURN_NONE;

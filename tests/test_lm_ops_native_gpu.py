@@ -144,3 +144,28 @@ def test_a_capture_beside_a_living_eager_graph_of_its_leaves_is_refused(name, fa
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want, strict=True))
+
+
+@pytest.mark.parametrize("name", ["qk_norm_rotary", "dropout", "embedding", "token_scores"])
+def test_traced_calls_compute_when_they_run(name):
+    """A recorded graph of a call gives the call's results for other inputs."""
+    inputs, call = _calls()[name]
+    with torch.no_grad():
+        traced = torch.jit.trace(lambda *a: tuple(t for t in call(*a) if t is not None), inputs, check_trace=False)
+        others = [torch.randn_like(t) for t in inputs]
+        for args in (inputs, others, inputs):
+            got, want = traced(*args), [t for t in call(*args) if t is not None]
+            assert len(got) == len(want) and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_the_extension_leaves_traced_calls():
+    from flash_pop_b200 import _lib
+    n, seen = _lib.native(), []
+    x, seed = torch.randn(5, 7, device="cuda"), torch.tensor([1], device="cuda")
+
+    def f(x):
+        seen.append((n.dropout(x, None, 0.5, seed), n.rotary(x.view(1, 5, 1, 7), None, x, False, x.dtype)))
+        return x * 2
+
+    torch.jit.trace(f, (x,), check_trace=False)
+    assert seen == [(None, None)] and n.dropout(x, None, 0.5, seed) is not None
