@@ -16,12 +16,22 @@ from flash_pop_b200.retnet import RetNetDecoder, RetNetDecoderLayer
 from flash_pop_b200.token_ops import TokenScores, embedding, token_scores
 
 
+def _plain_embedding(m: nn.Module) -> bool:
+    """An ``nn.Embedding`` whose rows are those of its weight, with nothing attached to it that a call would reach."""
+    if type(m) is not nn.Embedding or m.max_norm is not None or m.sparse or m.scale_grad_by_freq or "forward" in m.__dict__:
+        return False
+    own, every = m.__dict__, nn.modules.module
+    return not any(own.get(h, True) for h in ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")) and not (
+        every._global_forward_hooks or every._global_forward_pre_hooks or every._global_backward_hooks or every._global_backward_pre_hooks)
+
+
 class RetNetLM(nn.Module):
     def __init__(self, vocab_size: int = 32000, num_layers: int = 12, num_heads: int = 8, head_dim: int = 128,
                  dim_feedforward: int = 4096, dropout: float = 0.0, device="cuda", dtype=torch.bfloat16, embed_scale: Optional[float] = None,
                  qk_norm: bool = False, counter_dropout: bool = False):
-        """embed_scale: the embedding's rows are multiplied by it, and its gradient is summed in a fixed order (None: a plain
-        ``nn.Embedding``).  qk_norm, counter_dropout: see RetNetDecoderLayer.Config."""
+        """embed_scale: the embedding's rows are multiplied by it, an id outside the table has a row of zeros, and the gradient is summed
+        in a fixed order (None: a plain ``nn.Embedding``; an embedding with hooks, or another module in its place, is called, and its gradient is
+        its own).  qk_norm, counter_dropout: see RetNetDecoderLayer.Config."""
         super().__init__()
         d_model = num_heads * head_dim
         cfg = RetNetDecoderLayer.Config(num_heads=num_heads, head_dim_v=head_dim, head_dim_qk=head_dim,
@@ -35,10 +45,18 @@ class RetNetLM(nn.Module):
         nn.init.normal_(self.embed.weight, std=d_model ** -0.5)
         nn.init.normal_(self.head.weight, std=d_model ** -0.5)
 
+    def _rows(self, tokens: torch.Tensor) -> torch.Tensor:
+        m = self.embed
+        if self.embed_scale is None:
+            return m(tokens)
+        if _plain_embedding(m):
+            return embedding(tokens, m.weight, self.embed_scale, m.padding_idx)
+        inside = (tokens >= 0) & (tokens < getattr(m, "num_embeddings", self.head.out_features))
+        return (m(tokens.masked_fill(~inside, 0)) * self.embed_scale).masked_fill(~inside.unsqueeze(-1), 0)
+
     def forward(self, tokens: torch.Tensor, recurrent_state: Optional[RecurrentState] = None):
         """tokens: (B, T) int64 -> logits (B, T, vocab), new RecurrentState."""
-        x = self.embed(tokens) if self.embed_scale is None else embedding(tokens, self.embed.weight, self.embed_scale)
-        x, state = self.decoder(x, recurrent_state)
+        x, state = self.decoder(self._rows(tokens), recurrent_state)
         return self.head(norm_in_fp32(self.norm, x)), state
 
     def loss(self, tokens: torch.Tensor) -> torch.Tensor:

@@ -209,3 +209,48 @@ def test_one_token_launch_leaves_normed_layers_to_the_layer_path():
         assert decoder_token(_model().eval().decoder, x, None, RetNetDecoderLayer, MultiScaleRetention) is None
         assert decoder_token(_model(dropout=0.3, qk_norm=False).eval().decoder, x, None, RetNetDecoderLayer, MultiScaleRetention) is not None
         assert decoder_token(_model(dropout=0.3, qk_norm=False).decoder, x, None, RetNetDecoderLayer, MultiScaleRetention) is None
+
+
+def _observe(module):
+    """Counts of a module's forward hooks."""
+    seen = {"pre": 0, "post": 0, "back": 0}
+    module.register_forward_pre_hook(lambda m, a: seen.__setitem__("pre", seen["pre"] + 1))
+    module.register_forward_hook(lambda m, a, y: seen.__setitem__("post", seen["post"] + 1))
+    module.register_full_backward_hook(lambda m, gi, go: seen.__setitem__("back", seen["back"] + 1))
+    return seen
+
+
+def test_what_is_attached_to_the_embedding_is_kept():
+    m, tokens = _model(), _tokens(T=30)
+    table = m.embed.weight
+    step = lambda t=tokens: torch.autograd.grad(m.score(t).logprob.sum(), [table])[0]
+    want, want_padded = step(), None
+    padded = tokens.clone()
+    padded[:, 20:] = -1
+    want_padded = step(padded)
+    # the padding id's row gets no gradient, and the others what they had
+    m.embed.padding_idx = int(tokens[0, 3])
+    got = step()
+    keep = torch.arange(999, device="cuda") != m.embed.padding_idx
+    assert bool((got[~keep] == 0).all()) and bool((want[~keep] != 0).any()) and torch.equal(got[keep], want[keep])
+    m.embed.padding_idx = None
+    # hooks see the module's call; ids outside the table stay rows of zeros (the scale apart from the lookup: gradients of rows are rounded)
+    seen = _observe(m.embed)
+    for ids, ref in ((tokens, want), (padded, want_padded)):
+        got = step(ids)
+        assert float((got.double() - ref.double()).norm() / ref.double().norm()) < 3e-2
+    assert seen == {"pre": 2, "post": 2, "back": 2}
+    # a module in its place is called
+    m = _model()
+
+    class Twice(torch.nn.Embedding):
+        def forward(self, ids):
+            return 2 * super().forward(ids)
+
+    twice = Twice(999, 128, device="cuda", dtype=BF)
+    twice.load_state_dict(m.embed.state_dict())
+    m.embed_scale /= 2
+    plain = m(tokens)[0]
+    m.embed = twice
+    m.embed_scale /= 2
+    assert torch.equal(m(tokens)[0], plain)                      # (powers of two)
