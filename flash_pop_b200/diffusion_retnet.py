@@ -37,7 +37,7 @@ class DiffusionRetNetDecoderLayer(nn.Module):
         chunk_size: int = 512  # accepted for compatibility; unused
         qk_norm: bool = False          # RMS norm of every head of q and k before the rotation, weights shared by the heads
         qk_norm_eps: float = 1e-6
-        counter_dropout: bool = False  # dropout without a stored mask (other masks than torch's for the same seed)
+        counter_dropout: bool = False  # dropout without a stored mask (other masks than torch's; while it drops, CUDA tensors only)
 
     def __init__(self, config: Config, xpos_embedder: Optional[XPos] = None) -> None:
         super().__init__()

@@ -222,7 +222,8 @@ def dropout(x: Tensor, p: float, seed: Tensor, residual: Optional[Tensor] = None
 class CounterDropout(torch.nn.Module):
     """``nn.Dropout`` on `dropout`: a seed from torch's generator for every call, no mask in memory, and the addition of a
     residual in the same pass.  Reproducible by ``torch.manual_seed`` (other masks than nn.Dropout's), under checkpointing and
-    in captured graphs, as far as torch's generator is."""
+    in captured graphs, as far as torch's generator is.  Where there is something to drop (training, p > 0) it takes what `dropout` takes,
+    CUDA tensors in bfloat16 or float32, and raises for others; the seed is a launch of its own before the dropout's."""
 
     def __init__(self, p: float = 0.5):
         super().__init__()

@@ -102,7 +102,7 @@ class MultiScaleRetention(nn.Module):
         chunk_size: int = 512  # accepted for compatibility; unused
         qk_norm: bool = False          # RMS norm of every head of q and k before the rotation, weights shared by the heads
         qk_norm_eps: float = 1e-6
-        counter_dropout: bool = False  # dropout without a stored mask (other masks than torch's for the same seed)
+        counter_dropout: bool = False  # dropout without a stored mask (other masks than torch's; while it drops, CUDA tensors only)
 
     def __init__(self, config: Config, xpos_embedder: Optional[XPos] = None):
         super().__init__()
@@ -237,7 +237,9 @@ class RetNetDecoderLayer(nn.Module):
         chunk_size: int = 512  # accepted for compatibility; unused
         qk_norm: bool = False          # RMS norm of every head of q and k before the rotation, weights shared by the heads
         qk_norm_eps: float = 1e-6
-        counter_dropout: bool = False  # dropout without a stored mask, added to the residual in one pass (other masks than torch's)
+        # Dropout without a stored mask (other masks than torch's; while it drops, CUDA tensors only).  In pre-norm layers the feed-forward's is
+        # added to the residual in the same pass, and in forward_chunkwise the retention's too.
+        counter_dropout: bool = False
 
     def __init__(self, config: Config, xpos_embedder: Optional[XPos] = None) -> None:
         super().__init__()

@@ -137,3 +137,17 @@ def test_eps_of_the_norms_is_checked(handle, anywhere):
             fp.RetNetDecoder(fp.RetNetDecoderLayer.Config(num_heads=2, head_dim_v=16, dim_feedforward=32, device="cpu", dtype=torch.float32, qk_norm=True,
                                                           qk_norm_eps=eps), 1)
     assert fwd(0.0) == NULL and bwd(0.0) == NULL
+
+
+def test_counter_dropout_is_for_cuda_tensors_of_two_types(anywhere, monkeypatch):
+    """What it cannot drop it refuses, with the same errors as the operator; in eval mode and at p = 0 it takes anything."""
+    m, x = layer_ops.CounterDropout(0.5), torch.randn(3, 4)
+    for t in (x.half(), x.double(), x.long()):
+        with pytest.raises(ValueError, match="bfloat16 or float32"):
+            m(t)
+        with pytest.raises(ValueError, match="bfloat16 or float32"):
+            m(t, t)
+        assert m.eval()(t) is t and m.train().active()
+    monkeypatch.undo()
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        m(x)
