@@ -212,3 +212,52 @@ def test_contiguous_tensors_that_are_not_aligned(dtype, fast, monkeypatch):
     ones = [torch.empty_strided((1, T, H, d), (7, H * d, d, 1), device="cuda", dtype=dtype).copy_(t[:1]) for t in (q, k, dyq, dyk)]
     assert all(t.is_contiguous() and t.stride(0) == 7 for t in ones)                     # an odd stride that no element uses
     assert all(torch.equal(a, b) for a, b in zip(step(*ones), step(q[:1], k[:1], dyq[:1], dyk[:1]), strict=True))
+
+
+def _items(B, T, Hq, Hk, d):
+    """How many pieces of work a tensor's launch is cut into, as the launch counts them: stretches of up to eight tokens a group of
+    lanes, one row or two heads of it at a time, 256 threads."""
+    lanes = 1
+    while lanes * 8 < d:
+        lanes *= 2
+    groups, H = 256 // lanes, max(Hq, Hk)
+    sets = (H + 1) // 2 if H > 1 else 1
+    block, rounds = min(sets, groups), 8
+    while True:
+        stretch = groups // block * rounds
+        items = B * -(-T // stretch) * -(-sets // block)
+        if items >= 296 or rounds == 1:
+            return items, rounds, -(-sets // block)
+        rounds //= 2
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("B,T,Hq,Hk,d", [(8, 4096, 8, 8, 128), (6, 9001, 5, 2, 64), (8, 2503, 17, 40, 256), (1, 4001, 33, 1, 200), (31, 20011, 1, 1, 16)])
+def test_launches_with_more_pieces_than_ctas(B, T, Hq, Hk, d, dtype):
+    """More than 592 pieces: a CTA takes several, its sums of the weights' gradients carried over; more heads than a CTA holds at once."""
+    from flash_pop_b200.layer_ops import qk_norm_rotary
+    items, rounds, blocks = _items(B, T, Hq, Hk, d)
+    assert items > 592 and rounds == 8 and (blocks > 1) == (d >= 200)
+    g = torch.Generator(device="cuda").manual_seed(d)
+    rnd = lambda *s, t=dtype: torch.randn(*s, generator=g, device="cuda").to(t)
+    ph, half = _phasors(1, T, d), HALF[dtype]
+    leaves = [rnd(B, T, Hq, d), rnd(B, T, Hk, d), 1 + 0.2 * rnd(d, t=F32), 1 + 0.2 * rnd(d, t=F32)]
+    leaves = [t.requires_grad_(True) for t in leaves]
+    y, dy = qk_norm_rotary(*leaves, ph, 1e-6), [rnd(B, T, Hq, d), rnd(B, T, Hk, d)]
+    grads = torch.autograd.grad(y, leaves, dy)
+    # additions behind one another in a weight's gradient: two heads of eight tokens a piece, a CTA's pieces, its groups of lanes, the CTAs'
+    # sums by 32 warps and then the warps'; and four operations in each term
+    chain = -(-items // 592) * 16 + 256 // min(d // 8, 32) + 592 // 32 + 1 + 32 + 4
+    for i in (0, 1):
+        x, w = leaves[i].detach().double(), leaves[2 + i].detach().double()
+        ref = _formula(x, w, ph, 1e-6)
+        # (as in _check)
+        assert bool(((y[i].double() - ref).abs() <= half * ref.abs() + 2.0 ** -20 * _row_max(ref) + 1e-30).all())
+        r = 1 / (x.pow(2).mean(-1, keepdim=True) + 1e-6).sqrt()
+        n, gr = x * r, _formula_back(dy[i].double(), ph)
+        gw = gr * w
+        ref = r * (gw - n * (gw * n).mean(-1, keepdim=True))
+        scale = r * _row_max(dy[i].double()) * 2 * float(w.abs().max())
+        assert bool(((grads[i].double() - ref).abs() <= half * ref.abs() + 2.0 ** -18 * scale).all())
+        terms = gr * n
+        assert bool(((grads[2 + i].double() - terms.sum((0, 1, 2))).abs() <= chain * 2.0 ** -24 * terms.abs().sum((0, 1, 2)) + 1e-30).all())
