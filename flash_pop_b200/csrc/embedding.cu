@@ -3,6 +3,7 @@
 // An id outside the table has a zero row and no part in the gradient, and so has the padding id in the gradient.
 // Bound by HBM: forward reads the rows in use and writes N rows, backward reads N rows and writes the dense table.  The
 // gradient has to put the ids in order first (else rows of one id are added by atomics, in another order every time).
+#include <algorithm>
 #include <atomic>
 
 #include "fpb_common.cuh"
@@ -65,8 +66,7 @@ __global__ void __launch_bounds__(THREADS) lookup_kernel(const __grid_constant__
 // The ids are brought into order with their positions by a stable radix sort, so that the rows of one id follow one another in
 // the order of their positions.  An id without a part (outside the table, or the padding) counts as V and comes last.
 constexpr int RADIX_BITS = 8, RADIX = 1 << RADIX_BITS, PER_THREAD = 8, MAX_TILES = 256;
-constexpr int TILE_THREADS = 512, SUB = TILE_THREADS * PER_THREAD;              // of the sort by many CTAs
-constexpr int ONE_THREADS = 1024, ONE = ONE_THREADS * PER_THREAD;               // of the sort by one CTA
+constexpr int TILE_THREADS = 512, SUB = TILE_THREADS * PER_THREAD;
 
 struct SortParams {
   const int64_t* tokens;       // first pass: the ids as the caller gave them
@@ -75,7 +75,7 @@ struct SortParams {
   uint32_t* counts;            // (tiles, RADIX)
   int64_t N, V, padding;
   int32_t tiles, subs;         // a tile is `subs` times SUB ids
-  int32_t shift, bits, passes; // of the digit; passes: of the one-CTA sort
+  int32_t shift, bits;         // of the digit
   uint4* zero; int64_t zero_units; void* zero_tail; int64_t zero_elements; int32_t element;      // the table's gradient, cleared on the side
 };
 
@@ -125,13 +125,14 @@ template <int T> struct Order {
     __syncthreads();
   }
   // Ranks of a warp's entries among those of the same digit; leaves in `before` how many of each digit the warp has.  Which lanes share a digit is
-  // found by a ballot for each of its bits.  One barrier.
-  __device__ void rank(const uint32_t (&d)[PER_THREAD], uint32_t (&r)[PER_THREAD]) {
+  // found by a ballot for each of its bits.  One barrier.  `each`: how many entries a thread has.
+  __device__ void rank(const uint32_t (&d)[PER_THREAD], uint32_t (&r)[PER_THREAD], int each = PER_THREAD) {
     const unsigned lower = (1u << (threadIdx.x & 31)) - 1u;
     uint32_t* mine = before[threadIdx.x >> 5];
     unsigned same[PER_THREAD];
 #pragma unroll
     for (int i = 0; i < PER_THREAD; ++i) {
+      if (i >= each) break;
       same[i] = __ballot_sync(0xffffffffu, d[i] < RADIX);
 #pragma unroll
       for (int b = 0; b < RADIX_BITS; ++b) {
@@ -142,6 +143,7 @@ template <int T> struct Order {
     }
 #pragma unroll
     for (int i = 0; i < PER_THREAD; ++i) {
+      if (i >= each) break;
       const bool real = d[i] < RADIX;
       if (real) r[i] = mine[d[i]] + __popc(same[i] & lower);
       __syncwarp();
@@ -223,50 +225,6 @@ __global__ void __launch_bounds__(TILE_THREADS) scatter_kernel(const __grid_cons
       if (d[i] < RADIX) p.out[order.at(d[i], r[i])] = e[i];
     __syncthreads();
   }
-}
-
-// All passes of up to ONE ids in the first CTA; the others clear the table.
-struct OneShared {
-  Order<ONE_THREADS> order;
-  uint2 moved[ONE];
-};
-__global__ void __launch_bounds__(ONE_THREADS) one_sort_kernel(const __grid_constant__ SortParams p) {
-  extern __shared__ __align__(16) unsigned char dynamic[];
-  OneShared& sh = *reinterpret_cast<OneShared*>(dynamic);
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (blockIdx.x > 0) {
-    clear_table<ONE_THREADS>(p, blockIdx.x - 1, gridDim.x - 1);
-    return;
-  }
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n0 = warp * 32 * PER_THREAD + lane;
-  uint2 e[PER_THREAD];
-  uint32_t d[PER_THREAD], r[PER_THREAD];
-#pragma unroll
-  for (int i = 0; i < PER_THREAD; ++i) e[i] = entry(p, min((int64_t)n0 + i * 32, p.N - 1));
-  for (int pass = 0; pass < p.passes; ++pass) {
-#pragma unroll
-    for (int i = 0; i < PER_THREAD; ++i) d[i] = n0 + i * 32 < p.N ? digit(p, e[i].x, pass * p.bits) : RADIX;
-    sh.order.clear();
-    sh.order.rank(d, r);
-    uint32_t all = 0;
-    if (threadIdx.x < RADIX) {
-#pragma unroll
-      for (int w = 0; w < ONE_THREADS / 32; ++w) all += sh.order.before[w][threadIdx.x];
-    }
-    uint32_t base = sh.order.scan(all);
-    sh.order.place(base);
-#pragma unroll
-    for (int i = 0; i < PER_THREAD; ++i)
-      if (d[i] < RADIX) sh.moved[sh.order.at(d[i], r[i])] = e[i];
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < PER_THREAD; ++i)
-      if (n0 + i * 32 < p.N) e[i] = sh.moved[n0 + i * 32];
-    __syncthreads();
-  }
-#pragma unroll
-  for (int i = 0; i < PER_THREAD; ++i)
-    if (n0 + i * 32 < p.N) p.out[n0 + i * 32] = e[i];
 }
 
 // ---- gradient: sums over the rows of an id --------------------------------------------------------------------------
@@ -399,6 +357,231 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constan
     if (col + c < p.D) to[c] = from_float<T>(f[c] * p.scale);
 }
 
+// ---- gradient of a few ids: one launch ------------------------------------------------------------------------------
+// A CTA has every share-th row of the table, FEW_COLUMNS columns of it (or several such tiles, for very wide rows), and all that happens to
+// them: it clears them, picks their ids from all N and puts them in order (in shared memory), and sums.  Rows next to one another belong to
+// different CTAs, as frequent ids often are neighbours.  The ordered ids are cut into a piece for each strand of eight threads,
+// whatever ids they hold; parts of a run that goes over pieces' ends meet in shared memory, in the order of the pieces.  What shares and
+// pieces are depends on N, V, D and the ids alone: the same bits every time.
+// The calls it is for wait for the host (a launch is 2 us there) and for latency: 5003 ids of 8001 rows of 333 fp32 take 19 us, 10 of them until
+// the ids are in order, where a sort, the sums and a join of windows as launches of their own took 24 and the call 6 us more on the host;
+// 8192 ids of 32000 x 1024 bf16 29 and 33, 64 of them 20 and 28 (the table's 66 MB alone 10), 8192 equal ids 47 and 45.
+constexpr int FEW_THREADS = 1024, STRAND = 8, STRANDS = FEW_THREADS / STRAND, FEW_COLUMNS = STRAND * 8, RANKED = 256;
+static_assert(FEW_THREADS * PER_THREAD == FPB_EMBEDDING_FEW, "an id is held by a thread from the start");
+
+struct FewParams {
+  const int64_t* tokens;
+  const void* dy; int64_t dy_stride;
+  void* dw;
+  int64_t V, padding;
+  int32_t N, D, share, tiles, bits, passes;
+  float scale;
+};
+struct FewShared {
+  Order<FEW_THREADS> order;
+  uint2 sorted[FPB_EMBEDDING_FEW];                                 // (row / share, position)
+  float part[2][STRANDS][FEW_COLUMNS];                             // of a run that began in an earlier piece; of one that goes on in a later one
+  uint32_t count[FEW_THREADS / 32];
+};
+
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(FEW_THREADS) few_grad_kernel(const __grid_constant__ FewParams p) {
+  constexpr int AHEAD_OF = WIDE && sizeof(T) == 2 ? 8 : 4;          // rows in flight: 32 registers
+  extern __shared__ __align__(16) unsigned char dynamic[];
+  FewShared& sh = *reinterpret_cast<FewShared*>(dynamic);
+  const int strand = threadIdx.x / STRAND, lane = threadIdx.x % STRAND, warp = threadIdx.x / 32, n0 = warp * 32 * PER_THREAD + threadIdx.x % 32;
+  const unsigned lower = (1u << threadIdx.x % 32) - 1u;
+  const uint32_t share = (uint32_t)p.share;
+  // a thread's columns of a tile: eight beside one another, or (c * STRAND + lane)
+  auto column = [&](int tile, int c) { return (int64_t)tile * FEW_COLUMNS + (WIDE ? lane * 8 + c : c * STRAND + lane); };
+  auto write = [&](int64_t row, int tile, const float (&f)[8]) {
+    T* to = (T*)p.dw + row * p.D;
+    if constexpr (WIDE) {
+      if (column(tile, 0) < p.D) store8(to + column(tile, 0), f);
+    } else {
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (column(tile, c) < p.D) to[column(tile, c)] = from_float<T>(f[c]);
+    }
+  };
+
+  uint2 e[PER_THREAD];
+  unsigned with[PER_THREAD];                       // lanes whose id is a row of this share
+  int found = 0;                                   // (of the warp)
+#pragma unroll
+  for (int i = 0; i < PER_THREAD; ++i) {
+    const int64_t t = p.tokens[min(n0 + i * 32, p.N - 1)];
+    const bool inside = n0 + i * 32 < p.N && t >= 0 && t < p.V && t != p.padding;
+    e[i] = make_uint2((uint32_t)t / share, (uint32_t)(n0 + i * 32));
+    with[i] = __ballot_sync(0xffffffffu, inside && (uint32_t)t % share == blockIdx.x);
+    found += __popc(with[i]);
+  }
+  if (threadIdx.x % 32 == 0) sh.count[warp] = (uint32_t)found;
+  // The share's rows are cleared: a strand a row, or where rows are not aligned a warp.
+  for (int tile = blockIdx.y; tile < p.tiles; tile += gridDim.y) {
+    constexpr int TEAM = WIDE ? STRAND : 32, UNIT = WIDE ? 16 / (int)sizeof(T) : 1;
+    const int64_t last = min((int64_t)(tile + 1) * FEW_COLUMNS, (int64_t)p.D);
+    for (int64_t row = blockIdx.x + (int64_t)(threadIdx.x / TEAM) * share; row < p.V; row += (int64_t)(FEW_THREADS / TEAM) * share) {
+#pragma unroll
+      for (int c = threadIdx.x % TEAM * UNIT; c < FEW_COLUMNS; c += TEAM * UNIT) {
+        const int64_t col = (int64_t)tile * FEW_COLUMNS + c;
+        if (col >= last) break;
+        T* to = (T*)p.dw + row * p.D + col;
+        if constexpr (WIDE) *reinterpret_cast<uint4*>(to) = make_uint4(0, 0, 0, 0); else *to = from_float<T>(0.0f);
+      }
+    }
+  }
+  __syncthreads();
+  {
+    const uint32_t mine = sh.count[threadIdx.x % 32];              // of 32 warps
+    uint32_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (threadIdx.x % 32 >= (unsigned)o) upto += x;
+    }
+    found = (int)__shfl_sync(0xffffffffu, upto, 31);               // (of all)
+    uint32_t at = __shfl_sync(0xffffffffu, upto - mine, warp);
+#pragma unroll
+    for (int i = 0; i < PER_THREAD; ++i) {
+      if (with[i] >> threadIdx.x % 32 & 1u) sh.sorted[at + __popc(with[i] & lower)] = e[i];
+      at += __popc(with[i]);
+    }
+  }
+  __syncthreads();
+  // They stand in the order of their positions.  Up to RANKED of them go to their places by counting, each with four threads or more, who goes
+  // before it: those in front with a key that is not larger, those behind with a smaller one.  More go by digits, as many a thread as
+  // it takes all threads.  By counting and by two digits: 255 of them 3.7 and 6 us, 500 7.9 and 6.4.
+  if (found <= RANKED) {
+    uint32_t* keys = &sh.order.before[0][0];
+    if (threadIdx.x < RANKED) keys[threadIdx.x] = (int)threadIdx.x < found ? sh.sorted[threadIdx.x].x : 0xffffffffu;
+    __syncthreads();
+    int per = FEW_THREADS / RANKED;
+    while (per < 32 && found * per * 2 <= FEW_THREADS) per *= 2;
+    const int i = threadIdx.x / per;
+    const uint2 own = i < found ? sh.sorted[i] : make_uint2(0, 0);
+    uint32_t before = 0;
+    const int group = i & ~3;                      // (four keys at a time, those of i's own group once more)
+    for (int j = threadIdx.x % per * 4; j < found; j += per * 4) {
+      const uint4 k = *reinterpret_cast<const uint4*>(keys + j);
+      const uint32_t limit = own.x + (j < group);
+      before += (k.x < limit) + (k.y < limit) + (k.z < limit) + (k.w < limit);
+    }
+    if (threadIdx.x % per == 0)
+      for (int j = group; j < i; ++j) before += keys[j] == own.x;
+    for (int o = 1; o < per; o *= 2) before += __shfl_xor_sync(0xffffffffu, before, o);
+    __syncthreads();
+    if (i < found && threadIdx.x % per == 0) sh.sorted[before] = own;
+    __syncthreads();
+  } else {
+    const int each = (found + FEW_THREADS - 1) / FEW_THREADS, first = warp * 32 * each + threadIdx.x % 32;
+    uint32_t d[PER_THREAD], r[PER_THREAD];
+    for (int pass = 0; pass < p.passes; ++pass) {
+#pragma unroll
+      for (int i = 0; i < PER_THREAD; ++i) {
+        const bool real = i < each && first + i * 32 < found;
+        if (real) e[i] = sh.sorted[first + i * 32];
+        d[i] = real ? (e[i].x >> pass * p.bits) & ((1u << p.bits) - 1u) : RADIX;
+      }
+      sh.order.clear();
+      sh.order.rank(d, r, each);
+      uint32_t all = 0;
+      if (threadIdx.x < RADIX) {
+#pragma unroll
+        for (int w = 0; w < FEW_THREADS / 32; ++w) all += sh.order.before[w][threadIdx.x];
+      }
+      uint32_t base = sh.order.scan(all);
+      sh.order.place(base);
+#pragma unroll
+      for (int i = 0; i < PER_THREAD; ++i)
+        if (d[i] < RADIX) sh.sorted[sh.order.at(d[i], r[i])] = e[i];
+      __syncthreads();
+    }
+  }
+
+  // (the barriers above are also between the clearing and what is written to the same rows now)
+  const int piece = (found + STRANDS - 1) / STRANDS, begin = min(strand * piece, found), end = min(begin + piece, found);
+  auto key = [&](int i) { return sh.sorted[i].x; };
+  auto goes_on = [&](int at) { return at < found && key(at) == key(at - 1); };     // the run before `at`
+  const bool starts_open = begin < end && begin > 0 && goes_on(begin);
+  for (int tile = blockIdx.y; tile < p.tiles; tile += gridDim.y) {
+    if (begin < end) {
+      uint32_t id = key(begin);
+      bool open = starts_open;
+      float acc[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) acc[c] = 0.0f;
+      auto finish = [&](bool on) {
+        if (open || on) {
+          float* to = sh.part[open ? 0 : 1][strand];
+#pragma unroll
+          for (int c = 0; c < 8; ++c) to[WIDE ? lane * 8 + c : c * STRAND + lane] = acc[c];
+        } else {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) acc[c] *= p.scale;
+          write(blockIdx.x + (int64_t)id * share, tile, acc);
+        }
+      };
+      for (int i = begin; i < end; i += AHEAD_OF) {
+        Raw8<T> rows[WIDE ? AHEAD_OF : 1];
+        T single[WIDE ? 1 : AHEAD_OF][8];
+#pragma unroll
+        for (int j = 0; j < AHEAD_OF; ++j) {
+          // (behind the piece its last row again, and of columns behind the end the last one: loads behind a branch would wait for one another)
+          const T* from = (const T*)p.dy + (int64_t)sh.sorted[min(i + j, end - 1)].y * p.dy_stride;
+          if constexpr (WIDE) {
+            read8(from + min(column(tile, 0), (int64_t)p.D - 8), rows[j]);
+          } else {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) single[j][c] = from[min(column(tile, c), (int64_t)p.D - 1)];
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < AHEAD_OF; ++j) {
+          if (i + j >= end) break;
+          if (key(i + j) != id) {
+            finish(false);
+            id = key(i + j);
+            open = false;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) acc[c] = 0.0f;
+          }
+          float f[8];
+          if constexpr (WIDE) {
+            unpack8(rows[j], f);
+          } else {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) f[c] = to_float(single[j][c]);
+          }
+#pragma unroll
+          for (int c = 0; c < 8; ++c) acc[c] += f[c];
+        }
+      }
+      finish(goes_on(end));
+    }
+    __syncthreads();
+    // the strand in whose piece a run begins that goes on adds up its parts
+    if (begin < end && goes_on(end) && !(starts_open && key(begin) == key(end - 1))) {
+      const uint32_t id = key(end - 1);
+      int last = end;                              // of the run
+      for (int step = 1 << 12; step; step /= 2)
+        if (last + step < found && key(last + step) == id) last += step;
+      float a[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) a[c] = sh.part[1][strand][WIDE ? lane * 8 + c : c * STRAND + lane];
+#pragma unroll 4
+      for (int s = strand + 1; s <= last / piece; ++s) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) a[c] += sh.part[0][s][WIDE ? lane * 8 + c : c * STRAND + lane];
+      }
+#pragma unroll
+      for (int c = 0; c < 8; ++c) a[c] *= p.scale;
+      write(blockIdx.x + (int64_t)id * share, tile, a);
+    }
+    __syncthreads();
+  }
+}
+
 // How a gradient is cut up, and where its scratch memory lies.
 struct GradPlan {
   int tiles, subs, passes, bits, window;
@@ -407,6 +590,10 @@ struct GradPlan {
 };
 GradPlan plan_grad(int64_t N, int64_t V, int D) {
   GradPlan g{};
+  if (N <= FPB_EMBEDDING_FEW) {
+    g.bytes = 16;                                  // (nothing in it)
+    return g;
+  }
   const int64_t subs = (N + SUB - 1) / SUB;
   g.subs = (int)((subs + MAX_TILES - 1) / MAX_TILES);
   g.tiles = (int)((subs + g.subs - 1) / g.subs);
@@ -434,32 +621,16 @@ template <typename T>
 cudaError_t table_grad(const GradPlan& g, SortParams s, SumParams q, bool wide, char* space, cudaStream_t stream, int* n_launched) {
   constexpr int CLEARING = 592;                    // CTAs
   uint2* buffers[2] = {(uint2*)(space + g.sorted[0]), (uint2*)(space + g.sorted[1])};
-  cudaError_t e;
-  if (q.N <= ONE) {
-    // (a CTA alone: its passes need no launch, 4 us each, between them)
-    static std::atomic<bool> configured[64];
-    int dev = 0;
-    if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
-    if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
-      if ((e = cudaFuncSetAttribute(one_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(OneShared))) != cudaSuccess) return e;
-      if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
-    }
-    s.out = buffers[0];
-    e = launch_kernel(one_sort_kernel, dim3(1 + CLEARING / 4), ONE_THREADS, sizeof(OneShared), false, s, stream);
-    *n_launched += 1;
-    q.sorted = buffers[0];
-  } else {
-    e = cudaSuccess;
-    for (int pass = 0; pass < g.passes && e == cudaSuccess; ++pass) {
-      s.in = pass == 0 ? nullptr : buffers[(pass - 1) & 1];
-      s.out = buffers[pass & 1];
-      s.shift = pass * g.bits;
-      e = launch_kernel(digit_counts_kernel, dim3(g.tiles), TILE_THREADS, 0, pass > 0, s, stream);
-      if (e == cudaSuccess) e = launch_kernel(scatter_kernel, dim3(g.tiles + (pass == 0 ? CLEARING : 0)), TILE_THREADS, 0, true, s, stream);
-      *n_launched += 2;
-    }
-    q.sorted = buffers[(g.passes - 1) & 1];
+  cudaError_t e = cudaSuccess;
+  for (int pass = 0; pass < g.passes && e == cudaSuccess; ++pass) {
+    s.in = pass == 0 ? nullptr : buffers[(pass - 1) & 1];
+    s.out = buffers[pass & 1];
+    s.shift = pass * g.bits;
+    e = launch_kernel(digit_counts_kernel, dim3(g.tiles), TILE_THREADS, 0, pass > 0, s, stream);
+    if (e == cudaSuccess) e = launch_kernel(scatter_kernel, dim3(g.tiles + (pass == 0 ? CLEARING : 0)), TILE_THREADS, 0, true, s, stream);
+    *n_launched += 2;
   }
+  q.sorted = buffers[(g.passes - 1) & 1];
   if (e != cudaSuccess) return e;
   const int64_t units = wide ? q.D / 8 : q.D;
   q.log_threads = 0;
@@ -475,6 +646,25 @@ cudaError_t table_grad(const GradPlan& g, SortParams s, SumParams q, bool wide, 
     *n_launched += 1;
   }
   return e;
+}
+
+template <typename T, bool WIDE> cudaError_t few_grad(FewParams p, cudaStream_t stream) {
+  static std::atomic<bool> configured[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
+    if ((e = cudaFuncSetAttribute(few_grad_kernel<T, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(FewShared))) != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
+  }
+  p.tiles = (p.D + FEW_COLUMNS - 1) / FEW_COLUMNS;
+  const int across = p.tiles < 148 ? p.tiles : 148;                // one CTA an SM
+  p.share = (int32_t)std::min<int64_t>(148 / across, p.V);
+  int bits = 1;
+  while ((p.V - 1) / p.share >> bits) ++bits;
+  p.passes = (bits + RADIX_BITS - 1) / RADIX_BITS;
+  p.bits = (bits + p.passes - 1) / p.passes;
+  return launch_kernel(few_grad_kernel<T, WIDE>, dim3((unsigned)p.share, (unsigned)across), FEW_THREADS, sizeof(FewShared), false, p, stream);
 }
 
 template <typename T>
@@ -506,10 +696,18 @@ int64_t embedding_workspace(int64_t N, int64_t V, int D) {
 int launch_embedding_grad(int dtype, int64_t N, int64_t V, int D, const int64_t* tokens, int64_t padding, float scale, const void* dy,
                           int64_t dy_stride, void* dw, void* workspace, cudaStream_t stream, int* n_launched) {
   const GradPlan g = plan_grad(N, V, D);
-  const int size = dtype == FPB_BF16 ? 2 : 4;
+  const int size = dtype == FPB_BF16 ? 2 : 4, vec = 16 / size;
+  const bool wide = D % 8 == 0 && (N <= 1 || dy_stride % vec == 0) && ((uintptr_t)dy | (uintptr_t)dw) % 16 == 0;
+  if (N <= FPB_EMBEDDING_FEW) {
+    const FewParams p{tokens, dy, dy_stride, dw, V, padding, (int32_t)N, D, 1, 1, 1, 1, scale};
+    const cudaError_t e = dtype == FPB_BF16 ? (wide ? few_grad<__nv_bfloat16, true>(p, stream) : few_grad<__nv_bfloat16, false>(p, stream))
+                                            : (wide ? few_grad<float, true>(p, stream) : few_grad<float, false>(p, stream));
+    *n_launched = 1;
+    return e == cudaSuccess ? FPB_OK : FPB_ERR_LAUNCH;
+  }
   SortParams s{};
   s.tokens = tokens; s.N = N; s.V = V; s.padding = padding;
-  s.tiles = g.tiles; s.subs = g.subs; s.bits = g.bits; s.passes = g.passes;
+  s.tiles = g.tiles; s.subs = g.subs; s.bits = g.bits;
   s.counts = (uint32_t*)((char*)workspace + g.counts);
   const int64_t bytes = V * D * size;
   s.element = size;
@@ -520,8 +718,6 @@ int launch_embedding_grad(int dtype, int64_t N, int64_t V, int D, const int64_t*
   SumParams q{};
   q.dy = dy; q.dy_stride = dy_stride; q.dw = dw; q.partial = (float*)((char*)workspace + g.partial);
   q.N = N; q.windows = g.windows; q.V = (uint32_t)V; q.D = D; q.pitch = (int32_t)g.pitch; q.W = g.window; q.scale = scale;
-  const int vec = 16 / size;
-  const bool wide = D % 8 == 0 && (N <= 1 || dy_stride % vec == 0) && ((uintptr_t)dy | (uintptr_t)dw) % 16 == 0;
   *n_launched = 0;
   const cudaError_t e = dtype == FPB_BF16 ? table_grad<__nv_bfloat16>(g, s, q, wide, (char*)workspace, stream, n_launched)
                                           : table_grad<float>(g, s, q, wide, (char*)workspace, stream, n_launched);

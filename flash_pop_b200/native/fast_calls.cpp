@@ -21,8 +21,10 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
 #include "../../include/flash_pop_b200.h"
@@ -704,38 +706,83 @@ std::vector<int64_t> with_last(at::IntArrayRef sizes, int64_t last) {
   shape.push_back(last);
   return shape;
 }
-struct Embedding : torch::autograd::Function<Embedding> {
-  static at::Tensor run(const at::Tensor& t, const at::Tensor& w, double scale) {
-    const int64_t stride = pitch(w), D = w.size(1);
-    Place here(w);
-    const at::Tensor y = make(with_last(t.sizes(), D), w, w.scalar_type());
-    ran(unlocked([&] {
-      return entry.embedding_fwd(t.numel(), w.size(0), (int32_t)D, code(w.scalar_type()), (const int64_t*)t.data_ptr(), w.data_ptr(), stride, (float)scale,
-                                 y.data_ptr(), here.stream);
-    }));
-    return y;
-  }
-  static variable_list forward(AutogradContext* ctx, const at::Tensor& t, const at::Tensor& w, double scale, int64_t padding) {
-    const at::Tensor y = run(t, w, scale);
+at::Tensor embedding_rows(const at::Tensor& t, const at::Tensor& w, double scale) {
+  const int64_t stride = pitch(w), D = w.size(1);
+  Place here(w);
+  const at::Tensor y = make(with_last(t.sizes(), D), w, w.scalar_type());
+  ran(unlocked([&] {
+    return entry.embedding_fwd(t.numel(), w.size(0), (int32_t)D, code(w.scalar_type()), (const int64_t*)t.data_ptr(), w.data_ptr(), stride, (float)scale,
+                               y.data_ptr(), here.stream);
+  }));
+  return y;
+}
+at::Tensor embedding_gradient(const at::Tensor& t, const at::Tensor& g, int64_t V, double scale, int64_t padding) {
+  const int64_t D = g.size(-1), N = t.numel();
+  Place here(g);
+  const at::Tensor dy = dense(g), dw = make({V, D}, dy, dy.scalar_type());
+  const int64_t need = entry.embedding_workspace(N, V, (int32_t)D);
+  const at::Tensor scratch = need > 16 ? make({need}, dy, at::kByte) : dw;         // (a few ids' is not touched)
+  ran_backward(entry.embedding_bwd(N, V, (int32_t)D, code(dy.scalar_type()), (const int64_t*)t.data_ptr(), padding, (float)scale, dy.data_ptr(), D,
+                                   dw.data_ptr(), scratch.data_ptr(), need, here.stream));
+  return dw;
+}
+// The node as compiled autograd takes it: Function's, whose forward is called for its node alone and computes nothing.
+struct CompiledEmbedding : torch::autograd::Function<CompiledEmbedding> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& t, const at::Tensor& w, double scale, int64_t padding) {
     ctx->save_for_backward({t});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["padding"] = padding;
     ctx->saved_data["V"] = w.size(0);
-    return {y};
+    return make(with_last(t.sizes(), w.size(1)), w, w.scalar_type());
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    at::NoGradGuard no_grad;
+    return {at::Tensor(), embedding_gradient(ctx->get_saved_variables()[0], g[0], ctx->saved_data["V"].toInt(), ctx->saved_data["scale"].toDouble(),
+                                             ctx->saved_data["padding"].toInt()), at::Tensor(), at::Tensor()};
+  }
+};
+// A node without Function's context, whose making and running are 4 of the 55 us that a lookup and its gradient would take on the host.
+struct Embedding : torch::autograd::Node {
+  torch::autograd::SavedVariable tokens;
+  double scale;
+  int64_t padding, V, D;
+  at::TensorOptions like;                        // of the table
+  mutable std::shared_ptr<torch::autograd::Node> compiled;
+
+  static at::Tensor run(const at::Tensor& t, const at::Tensor& w, double scale, int64_t padding) {
+    at::Tensor y = embedding_rows(t, w, scale);
+    const std::shared_ptr<Embedding> node(new Embedding(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(t, w));
+    node->tokens = torch::autograd::SavedVariable(t, false);
+    node->scale = scale; node->padding = padding; node->V = w.size(0); node->D = w.size(1);
+    node->like = w.options().requires_grad(false);
+    torch::autograd::set_history(y, node);
+    return y;
+  }
+  std::string name() const override { return "EmbeddingBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    tokens.reset_data();
+    compiled.reset();
+  }
+  variable_list apply(variable_list&& g) override {
+    std::lock_guard<std::mutex> lock(mutex_);
     const bool graph = at::GradMode::is_enabled();
     at::NoGradGuard no_grad;
     may_be_captured();
-    const at::Tensor t = ctx->get_saved_variables()[0];
-    const int64_t V = ctx->saved_data["V"].toInt(), D = g[0].size(-1), N = t.numel();
-    Place here(g[0]);
-    const at::Tensor dy = dense(g[0]), dw = make({V, D}, dy, dy.scalar_type());
-    const int64_t need = entry.embedding_workspace(N, V, (int32_t)D);
-    const at::Tensor scratch = make({need}, dy, at::kByte);
-    ran_backward(entry.embedding_bwd(N, V, (int32_t)D, code(dy.scalar_type()), (const int64_t*)t.data_ptr(), ctx->saved_data["padding"].toInt(),
-                                     (float)ctx->saved_data["scale"].toDouble(), dy.data_ptr(), D, dw.data_ptr(), scratch.data_ptr(), need, here.stream));
-    return once({at::Tensor(), dw, at::Tensor(), at::Tensor()}, graph);
+    const at::Tensor t = tokens.unpack();        // (raises where it was freed or changed)
+    return once({at::Tensor(), g[0].defined() ? embedding_gradient(t, g[0], V, scale, padding) : at::Tensor()}, graph);
+  }
+  void compiled_args(torch::dynamo::autograd::CompiledNodeArgs& args) const override {
+    if (!compiled) {
+      at::AutoGradMode grad(true);
+      const at::Tensor w = at::empty({1, 1}, like).expand({V, D}).requires_grad_(true);       // (its shape counts)
+      compiled = CompiledEmbedding::apply(tokens.unpack(), w, scale, padding).grad_fn();
+    }
+    compiled->compiled_args(args);
+  }
+  variable_list apply_with_saved(const variable_list& inputs, torch::dynamo::autograd::SwapSavedVariables& saved) override {
+    return compiled->apply_with_saved(inputs, saved);
   }
 };
 // embedding(tokens, weight, scale, padding) -> (y,)
@@ -746,8 +793,7 @@ PyObject* embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t padding = integer(a[3]);
     NEED(real(w.scalar_type()) && w.dim() == 2 && w.size(1) <= 1 << 20);
     pitch(w);
-    if (graph_wanted({w})) return Embedding::apply(t, w, scale, padding);
-    return {Embedding::run(t, w, scale)};
+    return {graph_wanted({w}) ? Embedding::run(t, w, scale, padding) : embedding_rows(t, w, scale)};
   });
 }
 

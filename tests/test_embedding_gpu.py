@@ -134,3 +134,64 @@ def test_two_captured_steps_and_another_stream():
         graphs[i].replay()
         torch.cuda.synchronize()
         assert torch.equal(held[i], want[i])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("N,V,D", [(8191, 5000, 64), (8192, 8001, 65), (8193, 8001, 64), (8192, 1, 40), (5003, 8001, 333), (33, 200_003, 63), (7, 1 << 20, 72),
+                                   (1000, 100, 1), (3000, 7, 1024), (8192, 24, 520), (257, 1500, 9608), (130, 90, 9601), (1, 5, 19_000)])
+def test_gradients_of_a_few_ids(N, V, D, dtype):
+    """Up to 8192 ids the gradient is one launch: tables of fewer rows than shares of it, tiles of 64 columns with a rest, more tiles than CTAs."""
+    g = torch.Generator(device="cuda").manual_seed(N + D)
+    t = torch.randint(0, V, (N,), generator=g, device="cuda")
+    _check(t, V, D, dtype, scale=0.75, padding=0)
+    # as words fall: a few ids in every piece, most of them rare
+    t = (V ** torch.rand(N, generator=g, device="cuda", dtype=torch.float64)).long() - 1
+    t[N // 3:N // 3 + N // 10] = -100
+    _check(t, V, D, dtype)
+
+
+@pytest.mark.parametrize("D", [8, 333, 1024])
+def test_runs_over_the_pieces_of_a_few_ids(D):
+    N, V = 8192, 4000
+    i = torch.arange(N, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(D)
+    for n in (1, 2, 127, 128, 129, 1000, N):                       # one run: a piece each of one row or more
+        _check(i[:n] * 0 + 3999, V, D, BF)
+    for ids in (i % 2 * 1000, i // 64, i // 65, i // 63 * 9, i % 3 * 148, (i > 5) * 17, (i == N - 1) * 8, i // 4096 * 24,
+                torch.where(i % 5 == 0, 11, i // 2 % V)):          # runs that end at, before and behind pieces' ends
+        order = torch.randperm(N, generator=g, device="cuda")
+        _check(ids, V, D, F32)
+        _check(ids[order], V, D, BF)
+
+
+def test_the_node_is_an_ordinary_one():
+    """Saved tensors through hooks, freed or changed ones, an absent gradient, a second derivative, and a backward pass that is compiled."""
+    from flash_pop_b200.token_ops import embedding
+    w = torch.randn(50, 16, device="cuda", requires_grad=True)
+    t = torch.randint(0, 50, (9,), device="cuda")
+    (want,) = torch.autograd.grad(embedding(t, w, 2.0).sum(), [w])
+    packed = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda x: packed.append(x.shape) or x.cpu(), lambda x: x.cuda()):
+        y = embedding(t, w, 2.0)
+    assert packed == [t.shape] and torch.equal(torch.autograd.grad(y.sum(), [w])[0], want)
+    y = embedding(t, w, 2.0)
+    y.sum().backward()
+    assert torch.equal(w.grad, want) and y.grad_fn.name() == "EmbeddingBackward"
+    with pytest.raises(RuntimeError, match="second time"):
+        y.sum().backward()
+    y = embedding(t, w, 2.0)
+    t += 0
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    (none,) = torch.autograd.grad(torch._C._functions.UndefinedGrad()(embedding(t, w)).sum(), [w], allow_unused=True)
+    assert none is None
+    with torch.autograd.detect_anomaly(check_nan=False):
+        (got,) = torch.autograd.grad(embedding(t, w, 2.0).sum(), [w])
+    assert torch.equal(got, want)
+    import torch._dynamo.compiled_autograd as compiled
+    for ids, table in ((t, w), (t, w), (torch.randint(0, 900, (3, 4000), device="cuda"), torch.randn(900, 8, device="cuda").to(BF).requires_grad_(True))):
+        (want,) = torch.autograd.grad(embedding(ids, table, 0.5, 3).sum(), [table])
+        table.grad = None
+        with compiled._enable(torch.compile(backend="eager")):
+            embedding(ids, table, 0.5, 3).sum().backward()
+        assert torch.equal(table.grad, want)
