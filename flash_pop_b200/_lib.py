@@ -97,7 +97,7 @@ def _native_command(out: str) -> list[str]:
     lib = os.path.join(root, "lib")
     return [shutil.which("g++") or "g++", "-std=c++17", "-O2", "-fPIC", "-shared", *(f"-I{d}" for d in include),
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", NATIVE_SOURCE, "-o", out, f"-L{lib}", f"-Wl,-rpath,{lib}",
-            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python"]
 
 
 def _native_stale() -> bool:
