@@ -239,7 +239,11 @@ struct ScoreParams {
 };
 
 constexpr int N = 4;                  // vectors of a thread in flight at a time, a tile
-constexpr int RECORDS = 512, CANDIDATES = 256, MAX_EDGES = 14, MAX_SPLIT = 8, FEW = 20;
+constexpr int RECORDS = 512, CANDIDATES = 256, MAX_EDGES = 14, MAX_SPLIT = 8;
+// Up to FEW alternatives the bound comes from 32 parts of the row, for more from 64: the top-th largest of n parts' maxima lets about n ln(n / (n - top))
+// elements of a tile through, 22 and 34 at 16 and 21 alternatives of 32 parts, 19 and 25 of 64, whose order costs a second sort.  With 32 and 64 parts:
+// 16384 rows of 32000 bf16 logits, 17, 20, 24 and 28 alternatives 254 and 251, 272 and 262, 295 and 278, 348 and 290 us.
+constexpr int FEW = 16;
 
 template <int WARPS> struct Sums {
   Stats parts[WARPS];
@@ -269,8 +273,8 @@ template <int NT, typename F> __device__ __forceinline__ void rank_keys(const ui
   }
 }
 
-// The maxima of the parts that the tiles seen are cut into, 32 or, where more than FEW alternatives are wanted, 64; one or two a lane
-// of every warp.  A part is the same threads' share of every tile.
+// The maxima of the parts that the tiles seen are cut into, 32 or, where more than FEW alternatives are wanted and there are more threads, 64;
+// one or two a lane of every warp.  A part is the same threads' share of every tile.
 struct Parts {
   uint32_t a = 0, b = 0;
 };
@@ -292,10 +296,10 @@ template <int NT> __device__ __forceinline__ void add_maxima(Parts& parts, float
   if (!few) parts.b = max(parts.b, group[32 + lane]);
 }
 // the top-th largest of them
-__device__ __forceinline__ uint32_t kth(const Parts& parts, int top) {
+template <int NT> __device__ __forceinline__ uint32_t kth(const Parts& parts, int top) {
   if (top == 1) return __reduce_max_sync(ALL, parts.a);
   uint32_t sorted = sort_warp(parts.a);
-  if (top > FEW) sorted = merge_sorted(sorted, sort_warp(parts.b));
+  if (NT > 32 && top > FEW) sorted = merge_sorted(sorted, sort_warp(parts.b));
   return __shfl_sync(ALL, sorted, top - 1);
 }
 
@@ -465,7 +469,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) scores_kernel(const __grid_cons
       if ((i & (i + 1)) == 0 && i != 1) {
         Parts parts;
         add_maxima<NT>(parts, mine, p.top <= FEW, sh.group[(__popc(i) + (i > 0)) & 1]);
-        least = kth(parts, p.top);
+        least = kth<NT>(parts, p.top);
         // (a bound as low as a mask's value: only what is above it, the rest of the choice is made below)
         masked = value_of(least) < SMALLEST;
         bound = value_of(least + masked);
@@ -602,7 +606,9 @@ template <typename T> cudaError_t scores(ScoreParams p, cudaStream_t stream) {
   // alternatives, with 64, 128 and 256 threads: 16384 rows of 32000 209, 223 and 264 us, 8192 rows 120 and 123, 1024 rows 31, 27 and 29, 300
   // rows 22, 16 and 16; 64 and 128: 16384 rows of 4000 74 and 82, 2048 rows equal, 4096 rows of 128000 211 and 193, and without
   // alternatives 16384 rows of 8192 61 and 68, 8192 rows of 32000 108 and 103.  A short row gets what holds it in one round of loads.
-  if (vectors <= 32 * N && p.top <= FEW) return scores<T, 32>(p, stream);
+  // A warp has 32 parts for any number of alternatives below 32; with 32 and 64 threads 65536 rows of 1000 with 20, 24, 28 and 31 alternatives take 115
+  // and 231, 133 and 250, 162 and 272, 236 and 288 us.
+  if (vectors <= 32 * N && p.top < 32) return scores<T, 32>(p, stream);
   if (vectors <= 64 * N || (p.rows >= 2048 && vectors <= 64 * N * (p.top ? 16 : 4))) return scores<T, 64>(p, stream);
   if (vectors <= 128 * N || p.rows >= 592) return scores<T, 128>(p, stream);
   // Very few rows: a row over a cluster of CTAs, a vector a thread at least, two CTAs an SM at most.  One CTA a row, two, four and eight:

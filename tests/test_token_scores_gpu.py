@@ -343,3 +343,17 @@ def test_many_rows_of_any_size(dtype):
     z[-299::8, 9:] = -5e9
     for top in (0, 8):
         _check(z, t, top)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("N,V", [(60, 40), (60, 511), (2100, 517), (60, 1023), (60, 1031), (2100, 4003), (60, 9001)])
+def test_more_alternatives_than_half_of_the_parts(N, V, dtype):
+    z, t = _logits(N, V, dtype, N + V + 2)
+    z[::6] = -math.inf
+    z[::12, V // 3:V // 3 + 18] = 1.0
+    z[1::6] = torch.arange(V, device="cuda").to(dtype)
+    z[2::6] = -0.5
+    z[3::6, 20:] = torch.finfo(dtype).min
+    z[4::18, 5] = math.nan
+    for top in (15, 16, 17, 20, 21, 24, 31, 32):
+        _check(z, t, top, grad=False)
