@@ -38,7 +38,8 @@ __device__ __forceinline__ uint4 philox(uint64_t counter, uint32_t k0, uint32_t 
 
 // GROUPS groups of eight elements a thread, a CTA's width apart.  WIDE: 16-byte accesses (pointers 16-byte aligned).
 // Four groups share the generator's keys and have their loads in flight together: 33.5M bf16 elements 31 us instead of 37 with one (134 MB,
-// 21 us at the copy rate), with a residual 39 either way (201 MB, 31 us); integer products are what it issues most.
+// 21 us at the copy rate), with a residual 39 either way (201 MB, 31 us).  Without one 64 % of the issue slots and two thirds of the copy rate are in use:
+// neither is full, and which wait is the rest is not known.
 constexpr int GROUPS = 4;
 template <typename T, bool WIDE, bool RES>
 __global__ void __launch_bounds__(THREADS) dropout_kernel(const __grid_constant__ DropoutParams p) {

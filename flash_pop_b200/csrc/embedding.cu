@@ -363,9 +363,9 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constan
 // different CTAs, as frequent ids often are neighbours.  The ordered ids are cut into a piece for each strand of eight threads,
 // whatever ids they hold; parts of a run that goes over pieces' ends meet in shared memory, in the order of the pieces.  What shares and
 // pieces are depends on N, V, D and the ids alone: the same bits every time.
-// The calls it is for wait for the host (a launch is 2 us there) and for latency: 5003 ids of 8001 rows of 333 fp32 take 19 us, 10 of them until
-// the ids are in order, where a sort, the sums and a join of windows as launches of their own took 24 and the call 6 us more on the host;
-// 8192 ids of 32000 x 1024 bf16 29 and 33, 64 of them 20 and 28 (the table's 66 MB alone 10), 8192 equal ids 47 and 45.
+// The calls it is for wait for the host (a launch is 3 to 4 us there) and for latency: between events around the call 5003 ids of 8001 rows of 333
+// fp32 take 25 us where a sort, the sums and a join of windows as launches of their own took 30, 8192 ids of 32000 x 1024 bf16 31 and 34, 64 of
+// them 21 and 28 (10 of which the 66 MB of zeros), 8192 equal ids 49 and 46; 9000 ids, by those launches, take 41.
 constexpr int FEW_THREADS = 1024, STRAND = 8, STRANDS = FEW_THREADS / STRAND, FEW_COLUMNS = STRAND * 8, RANKED = 256;
 static_assert(FEW_THREADS * PER_THREAD == FPB_EMBEDDING_FEW, "an id is held by a thread from the start");
 
