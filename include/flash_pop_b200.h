@@ -366,7 +366,7 @@ int fpb_dropout(int64_t n, int32_t dtype, double p, const int64_t* seed, const v
  *   d_weight[v] = scale * sum of d_y[n] over the n with tokens[n] == v, in the order of n
  * (D at most 2^20) with fp32 sums, rounded once; ids outside the table and `padding` (-1: none) have no part.  The same bits every time.
  * `workspace`: fpb_embedding_workspace bytes, 16-byte aligned, used during the call only; for up to FPB_EMBEDDING_FEW ids, whose gradient is
- * one launch, its 16 bytes are neither read nor written.
+ * made in one launch (two for large tables), its 16 bytes are neither read nor written.
  */
 #define FPB_EMBEDDING_FEW 8192
 int fpb_embedding_fwd(int64_t N, int64_t V, int32_t D, int32_t dtype, const int64_t* tokens, const void* weight, int64_t w_stride,

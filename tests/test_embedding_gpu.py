@@ -195,3 +195,24 @@ def test_the_node_is_an_ordinary_one():
         with compiled._enable(torch.compile(backend="eager")):
             embedding(ids, table, 0.5, 3).sum().backward()
         assert torch.equal(table.grad, want)
+
+
+@pytest.mark.parametrize("N,V,D,dtype", [(100, 131_072, 63, F32), (100, 131_073, 63, F32), (3000, 65_536, 100, BF), (3000, 65_537, 100, BF), (8192, 300_001, 5, BF),
+                                         (500, 1 << 20, 8, BF), (500, (1 << 20) + 1, 8, F32), (1, 530_000, 72, BF), (8192, 200_000, 333, F32)])
+def test_tables_on_both_sides_of_where_they_are_cleared_first(N, V, D, dtype):
+    g = torch.Generator(device="cuda").manual_seed(V + N)
+    _check(torch.randint(0, V, (N,), generator=g, device="cuda"), V, D, dtype)
+    _check(torch.full((N,), -1, device="cuda"), V, D, dtype)                           # nobody writes: zeros alone, whatever was there
+
+
+def test_what_follows_a_gradient_waits_for_its_clearing():
+    """A large table cleared by a launch of its own, and no id that anything waits for: what reads the result next sees zeros."""
+    from flash_pop_b200.token_ops import embedding
+    w = torch.zeros(3_000_000, 33, device="cuda", dtype=BF, requires_grad=True)
+    t, dy = torch.full((5,), -1, device="cuda"), torch.ones(5, 33, device="cuda", dtype=BF)
+    for _ in range(5):
+        junk = torch.full((3_000_000, 33), 7.0, device="cuda", dtype=BF)                # (the memory that the gradient gets)
+        del junk
+        (got,) = torch.autograd.grad(embedding(t, w), [w], dy)
+        assert float(got.abs().max()) == 0
+        del got
