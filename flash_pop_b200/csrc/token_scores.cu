@@ -241,7 +241,7 @@ struct ScoreParams {
 constexpr int N = 4;                  // vectors of a thread in flight at a time, a tile
 constexpr int RECORDS = 512, CANDIDATES = 256, MAX_EDGES = 14, MAX_SPLIT = 8;
 // Up to FEW alternatives the bound comes from 32 parts of the row, for more from 64: the top-th largest of n parts' maxima lets about n ln(n / (n - top))
-// elements of a tile through, 22 and 34 at 16 and 21 alternatives of 32 parts, 19 and 25 of 64, whose order costs a second sort.  With 32 and 64 parts:
+// elements of a tile through, 22 and 34 at 16 and 21 alternatives of 32 parts, 18 and 25 of 64, whose order costs a second sort.  With 32 and 64 parts:
 // 16384 rows of 32000 bf16 logits, 17, 20, 24 and 28 alternatives 254 and 251, 272 and 262, 295 and 278, 348 and 290 us.
 constexpr int FEW = 16;
 
