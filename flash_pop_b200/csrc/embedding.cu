@@ -359,10 +359,10 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constan
 
 // ---- gradient of a few ids: one launch ------------------------------------------------------------------------------
 // A CTA has every share-th row of the table, FEW_COLUMNS columns of it (or several such tiles, for very wide rows), and all that happens to
-// them: it clears them (but for large tables), picks their ids from all N and puts them in order (in shared memory), and sums.  Rows next to one another belong to
-// different CTAs, as frequent ids often are neighbours.  The ordered ids are cut into a piece for each strand of eight threads,
-// whatever ids they hold; parts of a run that goes over pieces' ends meet in shared memory, in the order of the pieces.  What shares and
-// pieces are depends on N, V, D and the ids alone: the same bits every time.
+// them: it clears them (but for large tables), picks their ids from all N, puts them in order in shared memory, and sums.  Rows next to one
+// another belong to different CTAs, as frequent ids often are neighbours.  The ordered ids are cut into a piece for each strand of eight
+// threads, whatever ids they hold; parts of a run that goes over pieces' ends meet in shared memory, in the order of the pieces.  What
+// shares and pieces are depends on N, V, D and the ids alone: the same bits every time.
 // The calls it is for wait for the host (a launch is 3 to 4 us there) and for latency: between events around the call 5003 ids of 8001 rows of 333
 // fp32 take 25 us where a sort, the sums and a join of windows as launches of their own took 30, 8192 ids of 32000 x 1024 bf16 31 and 34, 64 of
 // them 21 and 28 (10 of which the 66 MB of zeros), 8192 equal ids 49 and 46; 9000 ids, by those launches, take 41.
@@ -386,7 +386,7 @@ struct FewShared {
 
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(FEW_THREADS) few_grad_kernel(const __grid_constant__ FewParams p) {
-  constexpr int AHEAD_OF = WIDE && sizeof(T) == 2 ? 8 : 4;          // rows in flight: 32 registers
+  constexpr int FLIGHT = WIDE && sizeof(T) == 2 ? 8 : 4;          // rows in flight: 32 registers
   extern __shared__ __align__(16) unsigned char dynamic[];
   FewShared& sh = *reinterpret_cast<FewShared*>(dynamic);
   const int strand = threadIdx.x / STRAND, lane = threadIdx.x % STRAND, warp = threadIdx.x / 32, n0 = warp * 32 * PER_THREAD + threadIdx.x % 32;
@@ -523,11 +523,11 @@ __global__ void __launch_bounds__(FEW_THREADS) few_grad_kernel(const __grid_cons
           write(blockIdx.x + (int64_t)id * share, tile, acc);
         }
       };
-      for (int i = begin; i < end; i += AHEAD_OF) {
-        Raw8<T> rows[WIDE ? AHEAD_OF : 1];
-        T single[WIDE ? 1 : AHEAD_OF][8];
+      for (int i = begin; i < end; i += FLIGHT) {
+        Raw8<T> rows[WIDE ? FLIGHT : 1];
+        T single[WIDE ? 1 : FLIGHT][8];
 #pragma unroll
-        for (int j = 0; j < AHEAD_OF; ++j) {
+        for (int j = 0; j < FLIGHT; ++j) {
           // (behind the piece its last row again, and of columns behind the end the last one: loads behind a branch would wait for one another)
           const T* from = (const T*)p.dy + (int64_t)sh.sorted[min(i + j, end - 1)].y * p.dy_stride;
           if constexpr (WIDE) {
@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(FEW_THREADS) few_grad_kernel(const __grid_cons
           }
         }
 #pragma unroll
-        for (int j = 0; j < AHEAD_OF; ++j) {
+        for (int j = 0; j < FLIGHT; ++j) {
           if (i + j >= end) break;
           if (key(i + j) != id) {
             finish(false);
